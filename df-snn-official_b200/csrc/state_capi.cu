@@ -1,0 +1,167 @@
+// state_capi.cu -- extern "C" entry points of the state-space layer (include/dfsnn_b200.h):
+// argument checks (nothing is launched on a bad call), workspace layout, launches.
+#include <climits>
+
+#include "kernels.h"
+#include "short_conv.h"
+#include "state_scan.h"
+
+namespace dfsnn {
+cudaError_t state_scan_step_launch(const dfsnn_state_scan_step_args& a, cudaStream_t st);
+}
+
+namespace {
+
+constexpr long long kMaxSteps = INT_MAX - 1024;     // tile arithmetic stays in 32 bits
+
+int status(cudaError_t e) { return e == cudaSuccess ? DFSNN_OK : dfsnn::record_cuda_error(e); }
+
+bool known_dtype(int d) {
+    return d == DFSNN_DTYPE_F32 || d == DFSNN_DTYPE_F16 || d == DFSNN_DTYPE_BF16;
+}
+bool flag(int v) { return v == 0 || v == 1; }
+
+int check_scan_sizes(long long T, long long batch, long long channels, int states, int groups) {
+    if (T < 1 || batch < 0 || channels < 0 || states < 1 || groups < 1) return DFSNN_ERR_SHAPE;
+    if (channels > INT_MAX - 1024 || channels % groups) return DFSNN_ERR_SHAPE;
+    if (T > kMaxSteps || states > DFSNN_SCAN_MAX_STATES) return DFSNN_ERR_T_LIMIT;
+    return DFSNN_OK;
+}
+
+int check_scan(const dfsnn_state_scan_args* a) {
+    if (!a) return DFSNN_ERR_NULL;
+    if (int s = check_scan_sizes(a->T, a->batch, a->channels, a->states, a->groups)) return s;
+    if (!known_dtype(a->dtype) || !flag(a->softplus) || !flag(a->lengths64)) return DFSNN_ERR_PARAM;
+    return DFSNN_OK;
+}
+
+dfsnn::ScanParams scan_params(const dfsnn_state_scan_args& a) {
+    dfsnn::ScanParams p{};
+    p.a = a;
+    p.T = (int)a.T;
+    p.group_channels = (int)(a.channels / a.groups);
+    return p;
+}
+
+struct ScanWorkspace {
+    int tiles, parts;
+    size_t bc, a, d;        // floats
+    size_t bytes() const { return (bc + a + d) * sizeof(float); }
+};
+
+ScanWorkspace scan_workspace(long long T, long long batch, long long channels, int states, int groups) {
+    ScanWorkspace w;
+    w.tiles = dfsnn::state_scan_bwd_tiles(states, channels / groups);
+    w.parts = dfsnn::state_scan_bwd_batch_parts(states, batch, channels / groups, groups);
+    w.bc = (size_t)2 * w.tiles * T * batch * groups * states;
+    w.a = (size_t)w.parts * channels * states;
+    w.d = (size_t)2 * w.parts * channels;
+    return w;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+size_t dfsnn_state_scan_kept_floats(long long T, long long batch, long long channels, int states) {
+    if (check_scan_sizes(T, batch, channels, states, 1)) return 0;
+    return (size_t)((T - 1) / DFSNN_SCAN_CHUNK) * batch * channels * states;
+}
+
+int dfsnn_state_scan_forward(const dfsnn_state_scan_args* a, void* stream) {
+    if (int s = check_scan(a)) return s;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->u || !a->delta || !a->A || !a->B || !a->C || !a->y) return DFSNN_ERR_NULL;
+    return status(dfsnn::state_scan_forward_launch(scan_params(*a), (cudaStream_t)stream));
+}
+
+size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,
+                                                int states, int groups) {
+    if (check_scan_sizes(T, batch, channels, states, groups) || batch == 0 || channels == 0) return 0;
+    return scan_workspace(T, batch, channels, states, groups).bytes();
+}
+
+int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    if (int s = check_scan(a)) return s;
+    if (!g) return DFSNN_ERR_NULL;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->u || !a->delta || !a->A || !a->B || !a->C || !g->grad_y || !g->grad_u || !g->grad_delta
+        || !g->grad_B || !g->grad_C || !g->grad_A)
+        return DFSNN_ERR_NULL;
+    if (!a->kept && a->T > DFSNN_SCAN_CHUNK) return DFSNN_ERR_NULL;
+    const ScanWorkspace w = scan_workspace(a->T, a->batch, a->channels, a->states, a->groups);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return DFSNN_ERR_WORKSPACE;
+    dfsnn::ScanParams p = scan_params(*a);
+    p.g = *g;
+    p.tiles = w.tiles;
+    p.batch_parts = w.parts;
+    p.part_bc = static_cast<float*>(workspace);
+    p.part_a = p.part_bc + w.bc;
+    p.part_d = p.part_a + w.a;
+    return status(dfsnn::state_scan_backward_launch(p, (cudaStream_t)stream));
+}
+
+int dfsnn_state_scan_step(const dfsnn_state_scan_step_args* a, void* stream) {
+    if (!a) return DFSNN_ERR_NULL;
+    if (int s = check_scan_sizes(1, a->batch, a->channels, a->states, a->groups)) return s;
+    if (a->slots < 0 || (!a->index && a->slots < a->batch)) return DFSNN_ERR_SHAPE;
+    if (!known_dtype(a->dtype) || !flag(a->softplus) || !flag(a->index64)) return DFSNN_ERR_PARAM;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->u || !a->delta || !a->A || !a->B || !a->C || !a->state || !a->state_out || !a->y)
+        return DFSNN_ERR_NULL;
+    return status(dfsnn::state_scan_step_launch(*a, (cudaStream_t)stream));
+}
+
+static int check_conv_sizes(long long T, long long batch, long long channels, int taps) {
+    if (T < 1 || batch < 0 || channels < 0 || channels > INT_MAX - 1024) return DFSNN_ERR_SHAPE;
+    if (T > kMaxSteps || taps < 1 || taps > DFSNN_CONV_MAX_TAPS) return DFSNN_ERR_T_LIMIT;
+    return DFSNN_OK;
+}
+
+static int check_conv(const dfsnn_short_conv_args* a) {
+    if (!a) return DFSNN_ERR_NULL;
+    if (int s = check_conv_sizes(a->T, a->batch, a->channels, a->taps)) return s;
+    if (!known_dtype(a->dtype) || !flag(a->silu) || !flag(a->lengths64)) return DFSNN_ERR_PARAM;
+    return DFSNN_OK;
+}
+
+int dfsnn_short_conv_forward(const dfsnn_short_conv_args* a, void* stream) {
+    if (int s = check_conv(a)) return s;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->x || !a->weight || !a->y) return DFSNN_ERR_NULL;
+    return status(dfsnn::short_conv_forward_launch(*a, (cudaStream_t)stream));
+}
+
+size_t dfsnn_short_conv_backward_workspace_size(long long T, long long batch, long long channels,
+                                                int taps) {
+    if (check_conv_sizes(T, batch, channels, taps) || batch == 0 || channels == 0) return 0;
+    return (size_t)dfsnn::short_conv_parts(T, batch, channels) * (taps + 1) * channels * sizeof(float);
+}
+
+int dfsnn_short_conv_backward(const dfsnn_short_conv_args* a, const dfsnn_short_conv_grads* g,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+    if (int s = check_conv(a)) return s;
+    if (!g) return DFSNN_ERR_NULL;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->x || !a->weight || !g->grad_y || !g->grad_x || !g->grad_weight) return DFSNN_ERR_NULL;
+    const size_t need = dfsnn_short_conv_backward_workspace_size(a->T, a->batch, a->channels, a->taps);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < need) return DFSNN_ERR_WORKSPACE;
+    return status(dfsnn::short_conv_backward_launch(*a, *g, static_cast<float*>(workspace),
+                                                    (cudaStream_t)stream));
+}
+
+int dfsnn_short_conv_step(const dfsnn_short_conv_step_args* a, void* stream) {
+    if (!a) return DFSNN_ERR_NULL;
+    if (int s = check_conv_sizes(1, a->batch, a->channels, a->taps)) return s;
+    if (a->slots < 0 || (!a->index && a->slots < a->batch)) return DFSNN_ERR_SHAPE;
+    if (!known_dtype(a->dtype) || !flag(a->silu) || !flag(a->index64)) return DFSNN_ERR_PARAM;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->x || !a->weight || !a->y) return DFSNN_ERR_NULL;
+    if (a->taps > 1 && (!a->state || !a->state_out)) return DFSNN_ERR_NULL;
+    return status(dfsnn::short_conv_step_launch(*a, (cudaStream_t)stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,104 @@
+// state_space.cuh -- shared device helpers of the state-space kernels (selective scan, short
+// causal convolution, and their single-token forms).
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../../include/dfsnn_b200.h"
+
+namespace dfsnn {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// element type <-> float (one rounding to nearest on the way out)
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename IO> __device__ __forceinline__ IO from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// 2^x by the hardware approximation (2 ulp; results below the normal range become 0)
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float sigmoid_f(float x) {
+    return __fdividef(1.0f, 1.0f + exp2_approx(-kLog2e * x));
+}
+
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|), which loses nothing at either end
+__device__ __forceinline__ float softplus_f(float x) {
+    return fmaxf(x, 0.0f) + log1pf(exp2_approx(-kLog2e * fabsf(x)));
+}
+
+// sequence length of row b: lengths[b] clamped to [0, T]; T without lengths
+__device__ __forceinline__ int seq_length(const void* lengths, int wide, long long b, int T) {
+    if (lengths == nullptr) return T;
+    const long long n = wide ? static_cast<const long long*>(lengths)[b]
+                             : static_cast<const int*>(lengths)[b];
+    return n < 0 ? 0 : (n > T ? T : (int)n);
+}
+
+// Sums each of CNT values over W lanes (lane = any + STRIDE * w, w = 0 .. W-1) by exchanging
+// halves: a stage sends the half of the values that the partner keeps, so W lanes need
+// CNT * (1 - 1/W) shuffles instead of CNT * log2 W.  Afterwards lane w holds, in
+// v[0 .. max(1, CNT / W) - 1], the sums of the values first(w) + i.
+template <int CNT, int W, int STRIDE>
+struct LaneSums {
+    static constexpr int kHeld = CNT >= W ? CNT / W : 1;
+    static __device__ __forceinline__ int first(int w) { return CNT >= W ? w * (CNT / W) : w / (W / CNT); }
+    // whether lane w is the one that stores (lanes share a sum when there are more lanes than values)
+    static __device__ __forceinline__ bool stores(int w) { return CNT >= W || w % (W >= CNT ? W / CNT : 1) == 0; }
+    static __device__ __forceinline__ void run(float (&v)[CNT], int w) {
+        int cnt = CNT;
+#pragma unroll
+        for (int m = W / 2; m >= 1; m >>= 1) {
+            if (cnt > 1) {
+                const int half = cnt / 2;
+                const bool up = (w & m) != 0;
+#pragma unroll
+                for (int i = 0; i < CNT / 2; ++i) {
+                    if (i < half) {
+                        const float send = up ? v[i] : v[i + half];
+                        const float keep = up ? v[i + half] : v[i];
+                        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m * STRIDE);
+                    }
+                }
+                cnt = half;
+            } else {
+                v[0] += __shfl_xor_sync(0xffffffffu, v[0], m * STRIDE);
+            }
+        }
+    }
+};
+
+// Slot of row b of a step call.  kIdle: a negative index; kBad: behind the last slot, or the slot
+// of an earlier row (two rows of one call cannot both advance it).  All threads of the block
+// call it together.
+constexpr long long kIdle = -1, kBad = -2;
+__device__ __forceinline__ long long index_at(const void* index, int wide, long long b) {
+    return wide ? static_cast<const long long*>(index)[b]
+                : (long long)static_cast<const int*>(index)[b];
+}
+__device__ __forceinline__ long long step_slot(const void* index, int wide, long long b,
+                                               long long slots) {
+    if (index == nullptr) return b;
+    const long long slot = index_at(index, wide, b);
+    bool taken = false;
+    if (slot >= 0)
+        for (long long r = threadIdx.x; r < b; r += blockDim.x)
+            taken |= index_at(index, wide, r) == slot;
+    taken = __syncthreads_or(taken);
+    if (slot < 0) return kIdle;
+    return taken || slot >= slots ? kBad : slot;
+}
+
+}  // namespace dfsnn

@@ -5,6 +5,7 @@ fallback: when it is missing or a call fails, the caller gets an exception.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "libdfsnn_b200.so")
@@ -30,6 +31,18 @@ _i = ctypes.c_int
 _ll = ctypes.c_longlong
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_args = ctypes.c_char_p      # a packed argument structure
+
+# The state-space entry points take their arguments as one packed structure (a bytes object laid
+# out as in the header: pointers, then 64-bit, then 32-bit fields), which costs a call much less
+# than two dozen converted arguments.
+STATE_SCAN_ARGS = struct.Struct("<13Q17q6i")
+STATE_SCAN_GRADS = struct.Struct("<11Q6q")
+STATE_SCAN_STEP_ARGS = struct.Struct("<12Q13q6i")
+SHORT_CONV_ARGS = struct.Struct("<7Q7q4i")
+SHORT_CONV_GRADS = struct.Struct("<6Q2q")
+SHORT_CONV_STEP_ARGS = struct.Struct("<7Q7q4i")
+SCAN_MAX_STATES, SCAN_CHUNK, CONV_MAX_TAPS = 128, 16, 8
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -76,6 +89,15 @@ SIGNATURES = {
                                    _i, _p, _sz, _p]),
     "dfsnn_vo_predictor_backward": (_i, [_p, _p, _p, _p, _p, _i, _i, _p, _p, _p, _p, _i, _ll, _f,
                                          _f, _f, _f, _p, _sz, _p]),
+    "dfsnn_state_scan_kept_floats": (_sz, [_ll, _ll, _ll, _i]),
+    "dfsnn_state_scan_forward": (_i, [_args, _p]),
+    "dfsnn_state_scan_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
+    "dfsnn_state_scan_backward": (_i, [_args, _args, _p, _sz, _p]),
+    "dfsnn_state_scan_step": (_i, [_args, _p]),
+    "dfsnn_short_conv_forward": (_i, [_args, _p]),
+    "dfsnn_short_conv_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i]),
+    "dfsnn_short_conv_backward": (_i, [_args, _args, _p, _sz, _p]),
+    "dfsnn_short_conv_step": (_i, [_args, _p]),
 }
 
 _lib = None

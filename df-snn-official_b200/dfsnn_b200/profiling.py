@@ -157,3 +157,23 @@ def euler_forward_bytes(T, N):
 
 def euler_backward_bytes(T, N):
     return N * (12 * T + 12)                     # x, grad_s in, grad_x out; z0, grad_zf in, grad_z0 out
+
+
+# state-space layer (elem: bytes of a sequence element; parameters and states float32)
+def state_scan_bytes(T, B, D, N, G, elem, gate, backward):
+    # forward: u, delta (z) in, y out; backward: u, delta (z), grad_y in, their gradients out
+    seqs = (4 if gate else 3) if not backward else (7 if gate else 5)
+    bc = (4 if backward else 2) * G * N
+    return T * B * elem * (seqs * D + bc) + D * N * 4 * (2 if backward else 1)
+
+
+def state_scan_step_bytes(B, D, N, G, elem, gate):
+    return B * (elem * ((4 if gate else 3) * D + 2 * G * N) + 8 * D * N) + 4 * D * N
+
+
+def short_conv_bytes(T, B, D, W, elem, backward):
+    return T * B * D * elem * (3 if backward else 2) + 4 * D * (W + 1) * (2 if backward else 1)
+
+
+def short_conv_step_bytes(B, D, W, elem):
+    return B * D * elem * 2 * W + 4 * D * (W + 1)

@@ -1,0 +1,509 @@
+"""State-space layer on B200: selective scan, short causal convolution and their step forms.
+
+The linear recurrence of state-space sequence models, beside this package's neuron
+recurrences and over the same time-major sequences, [T, B, D] (T steps, B sequences, D
+channels):
+
+  short_conv       p_t = bias + sum_j weight[:, j] x_(t-W+1+j);  y = p or silu(p)
+  state_scan       d_t = softplus(delta_t + delta_bias)
+                   h_t = exp(d_t A) h_(t-1) + d_t u_t B_t        (N states for each channel)
+                   y_t = (C_t . h_t + D u_t) silu(z_t)
+  short_conv_step, state_scan_step: one token for each row of a batch, on states that the
+                   caller keeps (one for each row, or a pool with an index)
+  StateSpaceLayer  the module around them: projections, convolution, scan
+
+The sequence forms are differentiable in every floating-point input.  Sequences are float32,
+float16 or bfloat16 (one type a call) with any strides over T and B, so halves of a projection
+and transposed batch-first tensors are read in place; outputs and gradients are dense in the
+order of the tensor they belong to.  Parameters, states and sums are float32.  There is no
+CPU path.
+
+All calls launch on the current stream of their tensors' device, wait for nothing and can be
+captured into a CUDA graph.  As with any torch operation, a backward can be captured only while
+no eager graph of the same leaves is alive (torch makes the leaves' gradient nodes wait for the
+stream of that graph, which a capture refuses): drop such outputs first.
+"""
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+from . import profiling as _prof
+
+_DTYPES = {torch.float32: _capi.DTYPE_F32, torch.float16: _capi.DTYPE_F16,
+           torch.bfloat16: _capi.DTYPE_BF16}
+_ACTIVATIONS = (None, "silu")
+
+
+# ---------------------------------------------------------------------------------------
+# argument checks
+# ---------------------------------------------------------------------------------------
+def _lead(x, name, dims):
+    """The sequence that sets a call's shape, type and device."""
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} requires CUDA tensors")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"{name}: float32, float16 or bfloat16 sequences, got {x.dtype}")
+    if x.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got {tuple(x.shape)}")
+    return _rows(x)
+
+
+def _rows(x):
+    return x if x.stride(-1) == 1 or x.size(-1) == 1 else x.contiguous()
+
+
+def _seq(x, like, shape, name, what):
+    """A further sequence of the call: same type and device, given shape, unit last stride."""
+    if x.dtype != like.dtype or x.device != like.device:
+        raise ValueError(f"{name}: {what} must be {like.dtype} on {like.device}, got {x.dtype} on {x.device}")
+    if x.shape != shape:
+        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    return _rows(x)
+
+
+def _param(x, device, shape, name, what):
+    """A float32 parameter or state (converted if need be), dense."""
+    if x is None:
+        return None
+    if x.device != device:
+        raise ValueError(f"{name}: {what} must be on {device}, got {x.device}")
+    if x.shape != shape:
+        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(x.shape)}")
+    if not x.dtype.is_floating_point:
+        raise ValueError(f"{name}: {what} must be floating-point, got {x.dtype}")
+    return (x if x.dtype == torch.float32 else x.float()).contiguous()
+
+
+def _integers(x, device, count, name, what):
+    if x is None:
+        return None
+    if x.dtype not in (torch.int32, torch.int64) or x.shape != (count,) or x.device != device:
+        raise ValueError(f"{name}: {what} must be int32 or int64 [{count}] on {device}, got "
+                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.contiguous()
+
+
+def _groups(x, like, lead, name, what):
+    """B or C as [..., G, N]; [..., N] is one group."""
+    if x.dim() == len(lead) + 1:
+        x = x.unsqueeze(-2)
+    if x.dim() != len(lead) + 2:
+        raise ValueError(f"{name}: {what} must be {tuple(lead)} + ([groups,] states), got {tuple(x.shape)}")
+    return _seq(x, like, (*lead, *x.shape[-2:]), name, what)
+
+
+def _scan_sizes(u, A, B, C, name):
+    D = u.shape[-1]
+    if A.dim() != 2 or A.shape[0] != D:
+        raise ValueError(f"{name}: A must have shape ({D}, states), got {tuple(A.shape)}")
+    N, G = A.shape[1], B.shape[-2]
+    if B.shape[-1] != N or C.shape != B.shape:
+        raise ValueError(f"{name}: B and C must agree and have {N} states, got {tuple(B.shape)} and "
+                         f"{tuple(C.shape)}")
+    if not 1 <= N <= _capi.SCAN_MAX_STATES:
+        raise ValueError(f"{name}: 1 to {_capi.SCAN_MAX_STATES} states, got {N}")
+    if G < 1 or D % G:
+        raise ValueError(f"{name}: {D} channels do not divide into {G} groups")
+    return D, N, G
+
+
+def _taps(weight, D, name):
+    if weight.dim() != 2 or weight.shape[0] != D:
+        raise ValueError(f"{name}: weight must have shape ({D}, taps), got {tuple(weight.shape)}")
+    W = weight.shape[1]
+    if not 1 <= W <= _capi.CONV_MAX_TAPS:
+        raise ValueError(f"{name}: 1 to {_capi.CONV_MAX_TAPS} taps, got {W}")
+    return W
+
+
+def _silu_flag(activation, name):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{name}: activation must be None or 'silu', got {activation!r}")
+    return int(activation == "silu")
+
+
+def _pool(state, state_out, device, dtype, inner, rows, index, name):
+    """(state, state_out, slots) of a step call.  Slots may lie anywhere along dimension 0 (one
+    layer of a pool for several), but each is dense: they are written in place."""
+    if state_out is None:
+        state_out = state
+    dense = (inner[1], 1)
+    for x, what in ((state, "state"), (state_out, "state_out")):
+        if x.dtype != dtype or x.device != device or x.dim() != 3 or x.shape[1:] != inner:
+            raise ValueError(f"{name}: {what} must be {dtype} [slots, {inner[0]}, {inner[1]}] on "
+                             f"{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        if x.numel() and x.stride()[1:] != dense and x.shape[1:] != (1, 1):
+            raise ValueError(f"{name}: each slot of {what} must be contiguous")
+        if x.shape[0] > 1 and x.stride(0) < inner[0] * inner[1]:
+            raise ValueError(f"{name}: the slots of {what} overlap")
+        if x.requires_grad:
+            raise ValueError(f"{name}: {what} is written in place and cannot require a gradient")
+    slots = state.shape[0]
+    if state_out.shape[0] != slots:
+        raise ValueError(f"{name}: state_out must have {slots} slots, got {state_out.shape[0]}")
+    if index is None and slots < rows:
+        raise ValueError(f"{name}: {rows} rows need as many slots, got {slots}")
+    if torch.is_grad_enabled() and not state_out.is_inference():
+        torch.autograd.graph.increment_version(state_out)
+    return state, state_out, slots
+
+
+# ---------------------------------------------------------------------------------------
+# calls
+# ---------------------------------------------------------------------------------------
+def _call(fn, name, launches, nbytes, device, *args):
+    """One native call on the current stream of `device`."""
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(fn, name, launches, nbytes, device, *args)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if _prof._ACTIVE is None:
+        code = fn(*args, stream)
+    else:
+        with _prof.native_call(name, launches, nbytes(), device):
+            code = fn(*args, stream)
+    if code:
+        _capi.check(code, name)
+
+
+def _p(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _tb(t):
+    return (0, 0) if t is None else (t.stride(0), t.stride(1))
+
+
+def _empty_like(x, zero=False):
+    """[T, B, D], dense, batch-first in memory where x is."""
+    T, B, D = x.shape
+    make = torch.zeros if zero else torch.empty
+    if T > 1 and B > 1 and x.stride(1) > x.stride(0):
+        return make((B, T, D), dtype=x.dtype, device=x.device).transpose(0, 1)
+    return make((T, B, D), dtype=x.dtype, device=x.device)
+
+
+def _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, y_strides, h_last, kept):
+    T, Bn, Dn = u.shape
+    return _capi.STATE_SCAN_ARGS.pack(
+        _p(u), _p(delta), _p(z), _p(B), _p(C), _p(A), _p(D), _p(bias), _p(h0), _p(lengths), _p(y),
+        _p(h_last), _p(kept), *_tb(u), *_tb(delta), *_tb(z), *B.stride()[:3], *C.stride()[:3],
+        *y_strides, T, Bn, Dn, A.shape[1], B.shape[2], _DTYPES[u.dtype], int(softplus),
+        int(lengths is not None and lengths.dtype == torch.int64), 0)
+
+
+def _scan_forward(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, want_last, keep):
+    T, Bn, Dn = u.shape
+    N = A.shape[1]
+    lib = _capi.lib()
+    y = _empty_like(u)
+    h_last = torch.empty((Bn, Dn, N), dtype=torch.float32, device=u.device) if want_last else None
+    kept = None
+    if keep:
+        count = lib.dfsnn_state_scan_kept_floats(T, Bn, Dn, N)
+        kept = torch.empty(count, dtype=torch.float32, device=u.device)
+    args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, _tb(y), h_last, kept)
+    _call(lib.dfsnn_state_scan_forward, "state_scan_forward", 1,
+          lambda: _prof.state_scan_bytes(T, Bn, Dn, N, B.shape[2], u.element_size(), z is not None, False),
+          u.device, args)
+    return y, h_last, kept
+
+
+class StateScanFunction(torch.autograd.Function):
+    """apply(u, delta, A, B, C, D, z, delta_bias, h0, lengths, softplus, return_state)
+    -> (y, last states or None); the arguments checked as by state_scan."""
+
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, bias, h0, lengths, softplus, want_last):
+        y, h_last, kept = _scan_forward(u, delta, A, B, C, D, z, bias, h0, lengths, softplus,
+                                        want_last, True)
+        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, h0, lengths, kept)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return y, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_last):
+        u, delta, A, B, C, D, z, bias, h0, lengths, kept = ctx.saved_tensors
+        T, Bn, Dn = u.shape
+        N, G = A.shape[1], B.shape[2]
+        dev, empty = u.device, Bn == 0 or Dn == 0
+        gy = _empty_like(u, zero=True) if grad_y is None else _rows(grad_y)
+        gl = None if grad_last is None else grad_last.float().contiguous()
+        gu, gdelta = _empty_like(u), _empty_like(delta)
+        gz = None if z is None else _empty_like(z)
+        gB, gC = (torch.empty((T, Bn, G, N), dtype=u.dtype, device=dev) for _ in range(2))
+        make = torch.zeros_like if empty else torch.empty_like
+        gA = make(A)
+        gD, gbias, gh0 = (None if x is None else make(x) for x in (D, bias, h0))
+        lib = _capi.lib()
+        args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, ctx.softplus, None, _tb(gy),
+                          None, kept)
+        grads = _capi.STATE_SCAN_GRADS.pack(
+            _p(gy), _p(gl), _p(gu), _p(gdelta), _p(gz), _p(gB), _p(gC), _p(gA), _p(gD), _p(gbias),
+            _p(gh0), *_tb(gu), *_tb(gdelta), *_tb(gz))
+        size = lib.dfsnn_state_scan_backward_workspace_size(T, Bn, Dn, N, G)
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        _call(lib.dfsnn_state_scan_backward, "state_scan_backward", 2,
+              lambda: _prof.state_scan_bytes(T, Bn, Dn, N, G, u.element_size(), z is not None, True),
+              dev, args, grads, ws.data_ptr(), ws.numel())
+        return gu, gdelta, gA, gB, gC, gD, gz, gbias, gh0, None, None, None
+
+
+def state_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=False, h0=None,
+               lengths=None, return_state=False):
+    """Selective scan over sequences.
+
+    u, delta, z [T, B, D]; A [D, N] (N <= 128); B, C [T, B, N] or, for G groups of D / G
+    neighbouring channels, [T, B, G, N]; D, delta_bias [D]; h0 [B, D, N] states in front of
+    step 0 (default zero).  d = delta (+ delta_bias), through softplus if asked; the gate
+    silu(z) multiplies the output where z is given.  lengths (int32 / int64 [B], on the
+    device): sequence b ends after lengths[b] steps; what its tensors hold behind is not
+    read, and outputs and gradients there are zero.  Returns y [T, B, D], with return_state
+    also the states after each sequence's last step, float32 [B, D, N]."""
+    name = "state_scan"
+    u = _lead(u, name, 3)
+    T, Bn, Dn = u.shape
+    if T < 1:
+        raise ValueError(f"{name}: at least one step, got T = {T}")
+    delta = _seq(delta, u, u.shape, name, "delta")
+    z = None if z is None else _seq(z, u, u.shape, name, "z")
+    B, C = _groups(B, u, (T, Bn), name, "B"), _groups(C, u, (T, Bn), name, "C")
+    _, N, _ = _scan_sizes(u, A, B, C, name)
+    A = _param(A, u.device, (Dn, N), name, "A")
+    D = _param(D, u.device, (Dn,), name, "D")
+    bias = _param(delta_bias, u.device, (Dn,), name, "delta_bias")
+    h0 = _param(h0, u.device, (Bn, Dn, N), name, "h0")
+    lengths = _integers(lengths, u.device, Bn, name, "lengths")
+    tensors = (u, delta, A, B, C, D, z, bias, h0)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        y, last = StateScanFunction.apply(*tensors, lengths, bool(softplus), bool(return_state))
+    else:
+        y, last, _ = _scan_forward(*tensors, lengths, softplus, return_state, False)
+    return (y, last) if return_state else y
+
+
+def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, softplus=False,
+                    index=None, state_out=None):
+    """One step of the selective scan for each of B rows; not differentiable.
+
+    u, delta, z [B, D]; B, C [B, N] or [B, G, N]; state float32 [S, D, N], a slot for each row
+    or, with index (int32 / int64 [B], on the device), a pool of S slots of which row b uses
+    index[b].  The new states replace the old ones, or go to the same slots of state_out.
+    A negative index marks an idle row: its y is zero and no state changes.  An index past
+    the pool, or one that an earlier row has, gives NaN and changes no state.  Returns
+    y [B, D]."""
+    name = "state_scan_step"
+    u = _lead(u, name, 2)
+    Bn, Dn = u.shape
+    delta = _seq(delta, u, u.shape, name, "delta")
+    z = None if z is None else _seq(z, u, u.shape, name, "z")
+    B, C = _groups(B, u, (Bn,), name, "B"), _groups(C, u, (Bn,), name, "C")
+    _, N, G = _scan_sizes(u, A, B, C, name)
+    dev = u.device
+    A = _param(A, dev, (Dn, N), name, "A")
+    D = _param(D, dev, (Dn,), name, "D")
+    bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
+    index = _integers(index, dev, Bn, name, "index")
+    state, state_out, slots = _pool(state, state_out, dev, torch.float32, (Dn, N), Bn, index, name)
+    y = torch.empty((Bn, Dn), dtype=u.dtype, device=dev)
+    args = _capi.STATE_SCAN_STEP_ARGS.pack(
+        _p(u), _p(delta), _p(z), _p(B), _p(C), _p(A), _p(D), _p(bias), _p(state), _p(state_out),
+        _p(index), _p(y), u.stride(0), delta.stride(0), 0 if z is None else z.stride(0),
+        B.stride(0), B.stride(1), C.stride(0), C.stride(1), Dn, state.stride(0),
+        state_out.stride(0), Bn, Dn, slots, N, G, _DTYPES[u.dtype], int(softplus),
+        int(index is not None and index.dtype == torch.int64), 0)
+    _call(_capi.lib().dfsnn_state_scan_step, name, 1,
+          lambda: _prof.state_scan_step_bytes(Bn, Dn, N, G, u.element_size(), z is not None), dev, args)
+    return y
+
+
+def _conv_args(x, weight, bias, state, lengths, silu, y, y_strides, last):
+    T, Bn, Dn = x.shape
+    return _capi.SHORT_CONV_ARGS.pack(
+        _p(x), _p(weight), _p(bias), _p(state), _p(lengths), _p(y), _p(last), *_tb(x), *y_strides,
+        T, Bn, Dn, weight.shape[1], _DTYPES[x.dtype], silu,
+        int(lengths is not None and lengths.dtype == torch.int64))
+
+
+def _conv_forward(x, weight, bias, state, lengths, silu, want_last):
+    T, Bn, Dn = x.shape
+    W = weight.shape[1]
+    y = _empty_like(x)
+    last = torch.empty((Bn, W - 1, Dn), dtype=x.dtype, device=x.device) if want_last else None
+    args = _conv_args(x, weight, bias, state, lengths, silu, y, _tb(y), last)
+    _call(_capi.lib().dfsnn_short_conv_forward, "short_conv_forward", 1,
+          lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), False), x.device, args)
+    return y, last
+
+
+class ShortConvFunction(torch.autograd.Function):
+    """apply(x, weight, bias, state, lengths, silu, return_state) -> (y, last inputs or None);
+    the arguments checked as by short_conv."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, silu, want_last):
+        y, last = _conv_forward(x, weight, bias, state, lengths, silu, want_last)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.silu = silu
+        ctx.set_materialize_grads(False)
+        return y, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_last):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        T, Bn, Dn = x.shape
+        W, dev = weight.shape[1], x.device
+        gy = _empty_like(x, zero=True) if grad_y is None else _rows(grad_y)
+        gl = None if grad_last is None else grad_last.contiguous()
+        gx = _empty_like(x)
+        make = torch.zeros_like if Bn == 0 or Dn == 0 else torch.empty_like
+        gw = make(weight)
+        gb, gs = (None if t is None else make(t) for t in (bias, state))
+        lib = _capi.lib()
+        args = _conv_args(x, weight, bias, state, lengths, ctx.silu, None, _tb(gy), None)
+        grads = _capi.SHORT_CONV_GRADS.pack(_p(gy), _p(gl), _p(gx), _p(gs), _p(gw), _p(gb), *_tb(gx))
+        size = lib.dfsnn_short_conv_backward_workspace_size(T, Bn, Dn, W)
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        _call(lib.dfsnn_short_conv_backward, "short_conv_backward", 2,
+              lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), True), dev, args, grads,
+              ws.data_ptr(), ws.numel())
+        return gx, gw, gb, gs, None, None, None
+
+
+def short_conv(x, weight, bias=None, activation=None, state=None, lengths=None, return_state=False):
+    """Causal convolution of each channel with a few taps.
+
+    x [T, B, D]; weight [D, W] (W <= 8; the last tap meets the current step); bias [D];
+    activation None or "silu"; state [B, W - 1, D], x's type: the inputs in front of step 0,
+    oldest first (default zero); lengths as in state_scan.  Returns y [T, B, D], with
+    return_state also the last W - 1 inputs of each sequence, for the tokens that follow."""
+    name = "short_conv"
+    silu = _silu_flag(activation, name)
+    x = _lead(x, name, 3)
+    T, Bn, Dn = x.shape
+    if T < 1:
+        raise ValueError(f"{name}: at least one step, got T = {T}")
+    W = _taps(weight, Dn, name)
+    weight = _param(weight, x.device, (Dn, W), name, "weight")
+    bias = _param(bias, x.device, (Dn,), name, "bias")
+    if state is not None:
+        state = _seq(state, x, (Bn, W - 1, Dn), name, "state").contiguous()
+    lengths = _integers(lengths, x.device, Bn, name, "lengths")
+    tensors = (x, weight, bias, state)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        y, last = ShortConvFunction.apply(*tensors, lengths, silu, bool(return_state))
+    else:
+        y, last = _conv_forward(*tensors, lengths, silu, return_state)
+    return (y, last) if return_state else y
+
+
+def short_conv_step(x, state, weight, bias=None, activation=None, index=None, state_out=None):
+    """One step of the short convolution for each of B rows; not differentiable.
+
+    x [B, D]; state [S, W - 1, D], x's type: the last inputs of each slot, oldest first, as
+    short_conv returns them; index and state_out as in state_scan_step.  Returns y [B, D]."""
+    name = "short_conv_step"
+    silu = _silu_flag(activation, name)
+    x = _lead(x, name, 2)
+    Bn, Dn = x.shape
+    W, dev = _taps(weight, Dn, name), x.device
+    weight = _param(weight, dev, (Dn, W), name, "weight")
+    bias = _param(bias, dev, (Dn,), name, "bias")
+    index = _integers(index, dev, Bn, name, "index")
+    state, state_out, slots = _pool(state, state_out, dev, x.dtype, (W - 1, Dn), Bn, index, name)
+    y = torch.empty((Bn, Dn), dtype=x.dtype, device=dev)
+    args = _capi.SHORT_CONV_STEP_ARGS.pack(
+        _p(x), _p(weight), _p(bias), _p(state), _p(state_out), _p(index), _p(y), x.stride(0), Dn,
+        state.stride(0), state_out.stride(0), Bn, Dn, slots, W, _DTYPES[x.dtype], silu,
+        int(index is not None and index.dtype == torch.int64))
+    _call(_capi.lib().dfsnn_short_conv_step, name, 1,
+          lambda: _prof.short_conv_step_bytes(Bn, Dn, W, x.element_size()), dev, args)
+    return y
+
+
+# ---------------------------------------------------------------------------------------
+# the layer
+# ---------------------------------------------------------------------------------------
+class StateSpaceLayer(nn.Module):
+    """Projections, short convolution and gated selective scan: [T, B, d_model] -> the same.
+
+    step_mode 'm' takes a whole sequence a call, 's' one step [B, d_model] a call, carrying its
+    states until reset(), as the neurons do.  Serving code that keeps its own states uses
+    forward(..., state=, return_state=True) for prompts and step() for tokens: a state is the
+    pair (convolution inputs [S, taps - 1, d_inner], scan states [S, d_inner, d_state])."""
+
+    def __init__(self, d_model, d_state=16, taps=4, expand=2, groups=1, rank=None, step_mode="m",
+                 step_range=(1e-3, 1e-1)):
+        super().__init__()
+        if step_mode not in ("s", "m"):
+            raise ValueError(f"step_mode must be 's' or 'm', got {step_mode!r}")
+        self.d_model, self.d_inner = int(d_model), int(expand * d_model)
+        self.d_state, self.groups, self.step_mode = int(d_state), int(groups), step_mode
+        if self.d_inner % self.groups:
+            raise ValueError(f"{self.d_inner} channels do not divide into {groups} groups")
+        self.rank = max(1, -(-self.d_model // 16)) if rank is None else int(rank)
+        self.in_proj = nn.Linear(self.d_model, 2 * self.d_inner, bias=False)
+        self.conv_weight = nn.Parameter(torch.empty(self.d_inner, taps).uniform_(-1, 1) / math.sqrt(taps))
+        self.conv_bias = nn.Parameter(torch.zeros(self.d_inner))
+        self.x_proj = nn.Linear(self.d_inner, self.rank + 2 * self.groups * self.d_state, bias=False)
+        self.dt_proj = nn.Linear(self.rank, self.d_inner, bias=False)
+        # softplus(delta_bias) is spread over step_range on a logarithmic scale
+        lo, hi = (math.log(v) for v in step_range)
+        step = torch.exp(torch.rand(self.d_inner) * (hi - lo) + lo)
+        self.delta_bias = nn.Parameter(torch.log(torch.expm1(step)))
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, self.d_state + 1, dtype=torch.float32))
+                                  .repeat(self.d_inner, 1))
+        self.D = nn.Parameter(torch.ones(self.d_inner))
+        self.out_proj = nn.Linear(self.d_inner, self.d_model, bias=False)
+        self.reset()
+
+    def reset(self):
+        self._state = None
+
+    def initial_state(self, slots, dtype=None, device=None):
+        w = self.in_proj.weight
+        dtype, device = dtype or w.dtype, device or w.device
+        return (torch.zeros(slots, self.conv_weight.shape[1] - 1, self.d_inner, dtype=dtype, device=device),
+                torch.zeros(slots, self.d_inner, self.d_state, device=device))
+
+    def _split(self, x):
+        dt, B, C = torch.split(self.x_proj(x), [self.rank, self.groups * self.d_state,
+                                                self.groups * self.d_state], dim=-1)
+        shape = (self.groups, self.d_state)
+        return self.dt_proj(dt), B.unflatten(-1, shape), C.unflatten(-1, shape)
+
+    def forward(self, x, lengths=None, state=None, return_state=False):
+        if self.step_mode == "s":
+            if lengths is not None or state is not None or return_state:
+                raise ValueError("step_mode 's' carries its own state: use step()")
+            return self.step(x, self._state)
+        conv0, h0 = (None, None) if state is None else state
+        x, z = self.in_proj(x).chunk(2, dim=-1)
+        x = short_conv(x, self.conv_weight, self.conv_bias, "silu", conv0, lengths, return_state)
+        if return_state:
+            x, conv0 = x
+        dt, B, C = self._split(x)
+        y = state_scan(x, dt, -torch.exp(self.A_log.float()), B, C, self.D, z, self.delta_bias, True,
+                       h0, lengths, return_state)
+        if return_state:
+            y, h0 = y
+        y = self.out_proj(y)
+        return (y, (conv0, h0)) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x, state, index=None):
+        """One token for each row of x [B, d_model]; state is advanced in place."""
+        x, z = self.in_proj(x).chunk(2, dim=-1)
+        if state is None:                       # the layer's own, from zero
+            state = self._state = self.initial_state(x.shape[0], x.dtype, x.device)
+        x = short_conv_step(x, state[0], self.conv_weight, self.conv_bias, "silu", index)
+        dt, B, C = self._split(x)
+        y = state_scan_step(x, dt, state[1], -torch.exp(self.A_log.float()), B, C, self.D, z,
+                            self.delta_bias, True, index)
+        return self.out_proj(y)

@@ -356,6 +356,160 @@ int dfsnn_gl_history_step_backward(int dtype, const void* grad_out, const void* 
 int dfsnn_check_surrogate_quotient(const float* a, int n_numerators, int exp_lo, int exp_hi,
                                    unsigned long long* mismatches, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * State-space layer: selective scan and short causal convolution (no reference counterpart)
+ *
+ * The linear recurrence that state-space sequence models put between their projections, next to
+ * this library's neuron recurrences, over the same time-major sequences.  T steps, `batch`
+ * sequences, `channels` channels; every sequence tensor has element (t, b, c) at
+ * t * x_t + b * x_b + c (strides in elements, channel stride 1), so halves of a wider
+ * projection and batch-first tensors are read in place.  `dtype` is the element type
+ * (DFSNN_DTYPE_*) of every sequence tensor of a call; parameters, states and their gradients
+ * are float32, and all sums are formed in float32.
+ *
+ * `lengths` (optional, int32 or, with lengths64, int64 [batch], device): sequence b has
+ * lengths[b] steps (clamped to 0..T).  Steps behind it are not read; their outputs and gradients
+ * are zero, and the last state is the one after step lengths[b] - 1 (the first state where the
+ * length is 0).
+ *
+ * The argument structures are read on the host before the call returns.
+ * ------------------------------------------------------------------------------- */
+
+#define DFSNN_SCAN_MAX_STATES 128   /* states per channel */
+#define DFSNN_SCAN_CHUNK 16         /* steps between the states that the forward keeps */
+#define DFSNN_CONV_MAX_TAPS 8
+
+/* Selective scan, per sequence b, channel c (of group c / (channels / groups)) and state n:
+ *   d_t = softplus(delta_t + delta_bias[c])   (softplus = 0: delta_t + delta_bias[c])
+ *   h_t[n] = exp(d_t * A[c][n]) * h_(t-1)[n] + d_t * u_t * B_t[n],   h_(-1) = h0 (NULL: 0)
+ *   o_t = sum_n C_t[n] * h_t[n] + D[c] * u_t                         (D NULL: without)
+ *   y_t = o_t, or o_t * z_t * sigmoid(z_t) with a gate z
+ * B and C have element (t, b, g, n) at t * B_t + b * B_b + g * B_g + n. */
+typedef struct {
+    const void* u;
+    const void* delta;
+    const void* z;              /* optional */
+    const void* B;
+    const void* C;
+    const float* A;             /* [channels, states] */
+    const float* D;             /* [channels], optional */
+    const float* delta_bias;    /* [channels], optional */
+    const float* h0;            /* [batch, channels, states], optional */
+    const void* lengths;        /* [batch], optional */
+    void* y;                    /* forward output */
+    float* h_last;              /* [batch, channels, states] last states, optional output */
+    float* kept;                /* dfsnn_state_scan_kept_floats() states for the backward: written
+                                   by the forward (optional), read by the backward */
+    long long u_t, u_b, delta_t, delta_b, z_t, z_b;
+    long long B_t, B_b, B_g, C_t, C_b, C_g, y_t, y_b;
+    long long T, batch, channels;
+    int states, groups, dtype, softplus, lengths64, reserved;
+} dfsnn_state_scan_args;
+
+/* Gradients: grad_y has y's strides; grad_u, grad_delta and grad_z their own; grad_B and grad_C are
+ * contiguous [T, batch, groups, states].  grad_h_last may be NULL (zero); grad_z, grad_D,
+ * grad_delta_bias and grad_h0 may be NULL where the input is NULL or the gradient is not wanted. */
+typedef struct {
+    const void* grad_y;
+    const float* grad_h_last;
+    void* grad_u;
+    void* grad_delta;
+    void* grad_z;
+    void* grad_B;
+    void* grad_C;
+    float* grad_A;
+    float* grad_D;
+    float* grad_delta_bias;
+    float* grad_h0;
+    long long gu_t, gu_b, gdelta_t, gdelta_b, gz_t, gz_b;
+} dfsnn_state_scan_grads;
+
+/* Floats of the `kept` array (the states at every DFSNN_SCAN_CHUNK steps; 0: none needed). */
+size_t dfsnn_state_scan_kept_floats(long long T, long long batch, long long channels, int states);
+int dfsnn_state_scan_forward(const dfsnn_state_scan_args* args, void* stream);
+size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,
+                                                int states, int groups);
+int dfsnn_state_scan_backward(const dfsnn_state_scan_args* args, const dfsnn_state_scan_grads* grads,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step for each of `batch` rows.  Row b reads the state at slot index[b] of `state` and
+ * writes the new one to the same slot of `state_out` (which may be `state`); without an index
+ * slot b is row b's.  A slot holds [channels, states] floats, slot s at s * state_s (out_s).
+ * index[b] < 0: an idle row, whose y is 0.  index[b] >= slots, or the slot of an earlier row:
+ * y is NaN and no state is touched.  Sequence tensors have element (b, c) at b * x_b + c. */
+typedef struct {
+    const void* u;
+    const void* delta;
+    const void* z;              /* optional */
+    const void* B;
+    const void* C;
+    const float* A;
+    const float* D;             /* optional */
+    const float* delta_bias;    /* optional */
+    const float* state;
+    float* state_out;
+    const void* index;          /* int32 or (index64) int64 [batch], optional */
+    void* y;
+    long long u_b, delta_b, z_b, B_b, B_g, C_b, C_g, y_b, state_s, out_s;
+    long long batch, channels, slots;
+    int states, groups, dtype, softplus, index64, reserved;
+} dfsnn_state_scan_step_args;
+
+int dfsnn_state_scan_step(const dfsnn_state_scan_step_args* args, void* stream);
+
+/* Short causal convolution per channel, `taps` weights:
+ *   p_t = bias[c] + sum_j weight[c][j] * x_(t - taps + 1 + j),   y_t = p_t, or p_t * sigmoid(p_t)
+ * x before step 0 is `state` [batch, taps - 1, channels], oldest first (NULL: zeros); `last`
+ * (optional) receives the last taps - 1 inputs of each sequence in the same layout.  Both have
+ * the sequences' type and are contiguous. */
+typedef struct {
+    const void* x;
+    const float* weight;        /* [channels, taps] */
+    const float* bias;          /* [channels], optional */
+    const void* state;          /* optional */
+    const void* lengths;        /* optional */
+    void* y;
+    void* last;                 /* optional */
+    long long x_t, x_b, y_t, y_b;
+    long long T, batch, channels;
+    int taps, dtype, silu, lengths64;
+} dfsnn_short_conv_args;
+
+/* grad_y has y's strides, grad_x its own; grad_last, grad_state [batch, taps - 1, channels] and
+ * grad_bias may be NULL. */
+typedef struct {
+    const void* grad_y;
+    const void* grad_last;
+    void* grad_x;
+    void* grad_state;
+    float* grad_weight;
+    float* grad_bias;
+    long long gx_t, gx_b;
+} dfsnn_short_conv_grads;
+
+int dfsnn_short_conv_forward(const dfsnn_short_conv_args* args, void* stream);
+size_t dfsnn_short_conv_backward_workspace_size(long long T, long long batch, long long channels,
+                                                int taps);
+int dfsnn_short_conv_backward(const dfsnn_short_conv_args* args, const dfsnn_short_conv_grads* grads,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step for each of `batch` rows; slots, index and refusals as in dfsnn_state_scan_step.  A
+ * slot holds the last taps - 1 inputs [taps - 1, channels], oldest first, in the sequences' type. */
+typedef struct {
+    const void* x;
+    const float* weight;
+    const float* bias;          /* optional */
+    const void* state;
+    void* state_out;
+    const void* index;          /* optional */
+    void* y;
+    long long x_b, y_b, state_s, out_s;
+    long long batch, channels, slots;
+    int taps, dtype, silu, index64;
+} dfsnn_short_conv_step_args;
+
+int dfsnn_short_conv_step(const dfsnn_short_conv_step_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
