@@ -19,6 +19,7 @@ int status(cudaError_t e) { return e == cudaSuccess ? DFSNN_OK : dfsnn::record_c
 bool known_dtype(int d) {
     return d == DFSNN_DTYPE_F32 || d == DFSNN_DTYPE_F16 || d == DFSNN_DTYPE_BF16;
 }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 bool flag(int v) { return v == 0 || v == 1; }
 
 int check_scan_sizes(long long T, long long batch, long long channels, int states, int groups) {
@@ -35,11 +36,21 @@ int check_scan(const dfsnn_state_scan_args* a) {
     return DFSNN_OK;
 }
 
+// Parts of the forward, and their floats in the workspace: [splits - 1] states and sums of d
+int forward_splits(const dfsnn_state_scan_args& a) {
+    return dfsnn::state_scan_splits(a.T, a.batch, a.channels / a.groups, a.groups, a.states);
+}
+size_t forward_floats(int splits, long long batch, long long channels, int states) {
+    return (size_t)(splits - 1) * batch * channels * (states + 1);
+}
+
 dfsnn::ScanParams scan_params(const dfsnn_state_scan_args& a) {
     dfsnn::ScanParams p{};
     p.a = a;
     p.T = (int)a.T;
     p.group_channels = (int)(a.channels / a.groups);
+    p.splits = 1;
+    p.split_steps = p.T;
     return p;
 }
 
@@ -59,8 +70,6 @@ ScanWorkspace scan_workspace(long long T, long long batch, long long channels, i
     return w;
 }
 
-bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
-
 }  // namespace
 
 extern "C" {
@@ -70,11 +79,31 @@ size_t dfsnn_state_scan_kept_floats(long long T, long long batch, long long chan
     return (size_t)((T - 1) / DFSNN_SCAN_CHUNK) * batch * channels * states;
 }
 
-int dfsnn_state_scan_forward(const dfsnn_state_scan_args* a, void* stream) {
+size_t dfsnn_state_scan_forward_workspace_size(long long T, long long batch, long long channels,
+                                               int states, int groups) {
+    if (check_scan_sizes(T, batch, channels, states, groups) || batch == 0 || channels == 0) return 0;
+    const int splits = dfsnn::state_scan_splits(T, batch, channels / groups, groups, states);
+    return forward_floats(splits, batch, channels, states) * sizeof(float);
+}
+
+int dfsnn_state_scan_forward(const dfsnn_state_scan_args* a, void* workspace, size_t workspace_bytes,
+                             void* stream) {
     if (int s = check_scan(a)) return s;
     if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
     if (!a->u || !a->delta || !a->A || !a->B || !a->C || !a->y) return DFSNN_ERR_NULL;
-    return status(dfsnn::state_scan_forward_launch(scan_params(*a), (cudaStream_t)stream));
+    dfsnn::ScanParams p = scan_params(*a);
+    p.splits = forward_splits(*a);
+    if (p.splits > 1) {
+        const size_t need = forward_floats(p.splits, a->batch, a->channels, a->states) * sizeof(float);
+        if (!workspace || !aligned16(workspace) || workspace_bytes < need) return DFSNN_ERR_WORKSPACE;
+        const long long chunks = (a->T + DFSNN_SCAN_CHUNK - 1) / DFSNN_SCAN_CHUNK;
+        const long long per = (chunks + p.splits - 1) / p.splits;
+        p.split_steps = (int)(per * DFSNN_SCAN_CHUNK);
+        p.ends = static_cast<float*>(workspace);
+        p.end_steps = p.ends + (size_t)(p.splits - 1) * a->batch * a->channels * a->states;
+        p.splits = (int)((chunks + per - 1) / per);
+    }
+    return status(dfsnn::state_scan_forward_launch(p, (cudaStream_t)stream));
 }
 
 size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,

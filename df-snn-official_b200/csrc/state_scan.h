@@ -13,6 +13,10 @@ struct ScanParams {
     dfsnn_state_scan_grads g;
     int T, group_channels;
     int tiles;                                 // channel tiles of a group
+    // a sequence in parts (splits > 1): `split_steps` steps each, a multiple of the chunk
+    int splits, split_steps;
+    float* ends;                               // [splits - 1][batch][channels][states]
+    float* end_steps;                          // [splits - 1][batch][channels] sums of d
     // backward
     int batch_parts;                           // blocks that share the batch (part q: b = q, q + parts, ...)
     float* part_bc;                            // [2][tiles][T][batch][groups][states]
@@ -20,6 +24,7 @@ struct ScanParams {
     float* part_d;                             // [2][batch_parts][channels] (D, delta_bias)
 };
 
+int state_scan_splits(long long T, long long batch, long long group_channels, int groups, int states);
 cudaError_t state_scan_forward_launch(const ScanParams& p, cudaStream_t st);
 int state_scan_bwd_tiles(int states, long long group_channels);
 int state_scan_bwd_batch_parts(int states, long long batch, long long group_channels, int groups);

@@ -37,7 +37,7 @@ template <typename IO, int S, int C, int SL, bool GATE>
 __global__ void __launch_bounds__(NT) scan_bwd(const ScanParams p) {
     using Sh = Shape<S, C, SL>;
     constexpr int CL = Sh::CL, NW = Sh::NW, BC = Sh::BC, NS = Sh::NS;
-    constexpr int E = (TT * BC + NT - 1) / NT, TS = NT / BC > 0 ? NT / BC : 1;
+    constexpr int E = (TT * BC + NT - 1) / NT, TS = TT / E;
     constexpr int F = (TT * NS + NT - 1) / NT;
     extern __shared__ __align__(16) float smem[];
     float(*s_dt)[P] = reinterpret_cast<float(*)[P]>(smem);

@@ -90,7 +90,8 @@ SIGNATURES = {
     "dfsnn_vo_predictor_backward": (_i, [_p, _p, _p, _p, _p, _i, _i, _p, _p, _p, _p, _i, _ll, _f,
                                          _f, _f, _f, _p, _sz, _p]),
     "dfsnn_state_scan_kept_floats": (_sz, [_ll, _ll, _ll, _i]),
-    "dfsnn_state_scan_forward": (_i, [_args, _p]),
+    "dfsnn_state_scan_forward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
+    "dfsnn_state_scan_forward": (_i, [_args, _p, _sz, _p]),
     "dfsnn_state_scan_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
     "dfsnn_state_scan_backward": (_i, [_args, _args, _p, _sz, _p]),
     "dfsnn_state_scan_step": (_i, [_args, _p]),

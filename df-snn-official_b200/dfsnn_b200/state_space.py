@@ -206,9 +206,11 @@ def _scan_forward(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, want_las
         count = lib.dfsnn_state_scan_kept_floats(T, Bn, Dn, N)
         kept = torch.empty(count, dtype=torch.float32, device=u.device)
     args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, _tb(y), h_last, kept)
-    _call(lib.dfsnn_state_scan_forward, "state_scan_forward", 1,
+    size = lib.dfsnn_state_scan_forward_workspace_size(T, Bn, Dn, N, B.shape[2])
+    ws = torch.empty(size, dtype=torch.uint8, device=u.device) if size else None
+    _call(lib.dfsnn_state_scan_forward, "state_scan_forward", 2 if size else 1,
           lambda: _prof.state_scan_bytes(T, Bn, Dn, N, B.shape[2], u.element_size(), z is not None, False),
-          u.device, args)
+          u.device, args, _p(ws), size)
     return y, h_last, kept
 
 

@@ -426,7 +426,11 @@ typedef struct {
 
 /* Floats of the `kept` array (the states at every DFSNN_SCAN_CHUNK steps; 0: none needed). */
 size_t dfsnn_state_scan_kept_floats(long long T, long long batch, long long channels, int states);
-int dfsnn_state_scan_forward(const dfsnn_state_scan_args* args, void* stream);
+/* Few long sequences are scanned in parts; their states need a workspace (0 bytes otherwise). */
+size_t dfsnn_state_scan_forward_workspace_size(long long T, long long batch, long long channels,
+                                               int states, int groups);
+int dfsnn_state_scan_forward(const dfsnn_state_scan_args* args, void* workspace,
+                             size_t workspace_bytes, void* stream);
 size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,
                                                 int states, int groups);
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* args, const dfsnn_state_scan_grads* grads,

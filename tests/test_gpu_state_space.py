@@ -118,6 +118,15 @@ def test_scan_batch_first_views():
     assert torch.autograd.grad(y.float().sum(), u)[0].shape == u.shape
 
 
+@pytest.mark.parametrize("T,B,D,N,G,lengths", [
+    (1000, 1, 40, 16, 1, None), (2049, 4, 36, 16, 2, [2049, 700, 0, 1]), (1500, 2, 12, 100, 1, [16, 1024]),
+    (999, 1, 130, 3, 1, None), (1040, 3, 9, 33, 3, [1040, 1039, 129])])
+def test_scan_in_parallel_parts(T, B, D, N, G, lengths):
+    """Few rows, many steps: parts of a sequence side by side."""
+    x, n, grads = scan_case(T, B, D, N, G, "f32", lengths=lengths, seed=T, scale=0.1)
+    check_scan(x, n, grads, True, f"parts {T}x{B}x{D}")
+
+
 def test_scan_large_batch_shares_blocks():
     """More sequences than the backward has blocks for: each block adds several."""
     x, n, grads = scan_case(3, 2500, 3, 4, 1, "f32", seed=6)

@@ -150,8 +150,19 @@ def scan_pack(**k):
     (dict(C=0), "NULL"), (dict(y=0), "NULL"), (dict(batch=0, u=0), "OK")])
 def test_scan_forward_refusals(change, code):
     f = _capi.lib().dfsnn_state_scan_forward
-    assert f(scan_pack(**change), None) == getattr(_capi, "DFSNN_OK" if code == "OK" else "DFSNN_ERR_" + code)
-    assert f(None, None) == _capi.DFSNN_ERR_NULL
+    assert f(scan_pack(**change), None, 0, None) == getattr(_capi, "DFSNN_OK" if code == "OK" else "DFSNN_ERR_" + code)
+    assert f(None, None, 0, None) == _capi.DFSNN_ERR_NULL
+
+
+def test_scan_forward_workspace():
+    """Few long sequences need one, and it is checked; many rows need none."""
+    L = _capi.lib()
+    size = L.dfsnn_state_scan_forward_workspace_size(8192, 1, 64, 16, 1)
+    assert size > 0 and L.dfsnn_state_scan_forward_workspace_size(8192, 512, 2048, 16, 1) == 0
+    assert L.dfsnn_state_scan_forward_workspace_size(16, 1, 64, 16, 1) == 0
+    long = scan_pack(T=8192, batch=1, channels=64)
+    for ws, n in ((None, size), (ctypes.c_void_p(0x1008), size), (ctypes.c_void_p(0x1000), size - 1)):
+        assert L.dfsnn_state_scan_forward(long, ws, n, None) == _capi.DFSNN_ERR_WORKSPACE
 
 
 def test_scan_backward_refusals():
