@@ -13,6 +13,7 @@ struct ScanParams {
     dfsnn_state_scan_grads g;
     int T, group_channels;
     int tiles;                                 // channel tiles of a group
+    bool words;                                // rows_aligned(4), for rows that are not on 16 bytes
     // a sequence in parts (splits > 1): `split_steps` steps each, a multiple of the chunk
     int splits, split_steps;
     float* ends;                               // [splits - 1][batch][channels][states]
@@ -23,6 +24,19 @@ struct ScanParams {
     float* part_a;                             // [batch_parts][channels][states]
     float* part_d;                             // [2][batch_parts][channels] (D, delta_bias)
 };
+
+// Whether every row (a step's channels of a group, a step's states) of the forward's inputs starts
+// on a multiple of `bytes`.  Channel tiles start on multiples of 4 channels, whole rows of a tile.
+inline bool rows_aligned(const ScanParams& p, size_t elem, size_t bytes) {
+    const dfsnn_state_scan_args& a = p.a;
+    auto ok = [&](const void* q, long long t, long long b, long long g) {
+        return reinterpret_cast<uintptr_t>(q) % bytes == 0 && t * (long long)elem % (long long)bytes == 0
+               && b * (long long)elem % (long long)bytes == 0 && g * (long long)elem % (long long)bytes == 0;
+    };
+    const long long gc = p.group_channels;
+    return ok(a.u, a.u_t, a.u_b, a.groups > 1 ? gc : 0) && ok(a.delta, a.delta_t, a.delta_b, 0)
+           && ok(a.z, a.z_t, a.z_b, 0) && ok(a.B, a.B_t, a.B_b, a.B_g) && ok(a.C, a.C_t, a.C_b, a.C_g);
+}
 
 int state_scan_splits(long long T, long long batch, long long group_channels, int groups, int states);
 cudaError_t state_scan_forward_launch(const ScanParams& p, cudaStream_t st);

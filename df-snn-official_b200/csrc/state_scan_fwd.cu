@@ -21,29 +21,44 @@
 #include <algorithm>
 
 #include "state_scan.h"
+#include "state_tile.cuh"
 
 namespace dfsnn {
 namespace {
 
-constexpr int TT = kScanChunk, S = 4, NT = 128;
+constexpr int TT = kScanChunk, NT = 128;
 
-template <int SL>
+// S states on each of a channel's SL lanes, C channels a lane
+template <typename IO, int S, int SL, int C>
 struct Tile {
-    static constexpr int CL = 32 / SL;                 // channels of a warp
-    static constexpr int BC = NT / 32 * CL;            // channels of the block
+    static constexpr int CL = 32 / SL;                 // channel lanes of a warp
+    static constexpr int CW = CL * C;                  // channels of a warp
+    static constexpr int BC = NT / 32 * CW;            // channels of the block
     static constexpr int NS = S * SL;                  // states, padded
-    static constexpr int E = CL > 1 ? CL / 2 : 1;      // (step, channel) elements of a thread,
-    static constexpr int TS = TT / E;                  // this many steps apart
-    static constexpr int F = (TT * NS + NT - 1) / NT;  // entries of B (and C) of a thread
-    float4 d[BC][TT + 1];                              // (d, d, d u, d u): packed operands as they are
-    float B[TT][NS], C[TT][NS];
-    float o[BC][TT + 4];
+    struct Raw {                                       // as the sequences have them
+        IO u[TT][BC], d[TT][BC], z[TT][BC], B[TT][NS], C_[TT][NS];
+    };
+    __align__(16) Raw raw[2];                          // this tile's and the next one's
+    float2 d[BC][TT + 1];                              // (d, d u)
+    __align__(16) float B[TT][NS], C_[TT][NS];
+    float o[BC][TT + 1];
 };
 
-template <typename IO, int SL, bool ENDS>
+// V neighbouring elements of a sequence
+template <typename IO, int V>
+struct __align__(sizeof(IO) * V) Pack {
+    IO v[V];
+};
+
+template <typename IO, int S, int SL, int C, bool WIDE, bool ENDS>
 __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
-    using Tl = Tile<SL>;
-    constexpr int CL = Tl::CL, BC = Tl::BC, NS = Tl::NS, E = Tl::E, F = Tl::F, TS = Tl::TS;
+    using Tl = Tile<IO, S, SL, C>;
+    constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS;
+    constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
+    constexpr int ROW = BC / V;                                 // threads along a step's channels
+    constexpr int E = TT * ROW > NT ? TT * ROW / NT : 1;        // packs of a thread,
+    constexpr int TS = TT / E;                                  // this many steps apart
+    using Elem = Pack<IO, V>;
     extern __shared__ __align__(16) unsigned char smem[];
     Tl& sh = *reinterpret_cast<Tl*>(smem);
     const dfsnn_state_scan_args& a = p.a;
@@ -65,213 +80,282 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
     const int c_base = tile * BC;                               // within the group
     const long long g_base = (long long)grp * p.group_channels; // first channel of the group
 
-    // elementwise role: elements (step t_e + e * TS, channel ch)
-    const int ch = tid % BC, t_e = tid / BC;
+    // elementwise role: elements (step t_e + e * TS, channels ch .. ch + V - 1)
+    const int ch = tid % ROW * V, t_e = tid / ROW;
     const bool ch_ok = c_base + ch < p.group_channels && t_e < TT;
     const long long chan = g_base + c_base + ch;
-    const float bias = ch_ok && a.delta_bias ? a.delta_bias[chan] : 0.0f;
-    const float skip = ch_ok && a.D ? a.D[chan] : 0.0f;
-    const IO* u_p = static_cast<const IO*>(a.u) + b * a.u_b + chan + (first + t_e) * a.u_t;
-    const IO* d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + chan + (first + t_e) * a.delta_t;
-    const IO* z_p = static_cast<const IO*>(a.z) + b * a.z_b + chan + (first + t_e) * a.z_t;
-    IO* y_p = static_cast<IO*>(a.y) + b * a.y_b + chan + (first + t_e) * a.y_t;
-    // entries of B and C: state n_f, steps t_f + f * DF
-    const int n_f = tid % NS, t_f = tid / NS;
-    constexpr int DF = NT / NS > 0 ? NT / NS : 1;               // steps between a thread's entries
-    const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + n_f + (first + t_f) * a.B_t;
-    const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + n_f + (first + t_f) * a.C_t;
-
-    // recurrence role: states n0 .. n0 + 3 of channel cl of the block
-    const int sl = lane % SL, cl = warp * CL + lane / SL, n0 = sl * S;
-    const bool cl_ok = c_base + cl < p.group_channels;
-    const long long row = ((long long)b * a.channels + g_base + c_base + cl) * a.states + n0;
-    // a lane's states are one float4 everywhere
-    const bool whole = a.states % S == 0
-                       && ((reinterpret_cast<uintptr_t>(a.kept) | reinterpret_cast<uintptr_t>(a.h_last)) & 15) == 0;
-    float2 A2[S / 2] = {}, h[S / 2] = {};
-    auto get = [&](const float* q, float2(&v)[S / 2]) {
-        float f[S];
+    float bias[V], skip[V];
 #pragma unroll
-        for (int s = 0; s < S; ++s) f[s] = q && cl_ok && n0 + s < a.states ? q[s] : 0.0f;
-        v[0] = make_float2(f[0], f[1]);
-        v[1] = make_float2(f[2], f[3]);
+    for (int v = 0; v < V; ++v) {
+        bias[v] = ch_ok && a.delta_bias ? a.delta_bias[chan + v] : 0.0f;
+        skip[v] = !ENDS && ch_ok && a.D ? a.D[chan + v] : 0.0f;
+    }
+    IO* y_p = static_cast<IO*>(a.y) + b * a.y_b + chan + (first + t_e) * a.y_t;
+    // the block's sequences at step `first`
+    const IO* u_p = static_cast<const IO*>(a.u) + b * a.u_b + g_base + c_base + first * a.u_t;
+    const IO* d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + g_base + c_base + first * a.delta_t;
+    const IO* z_p = static_cast<const IO*>(a.z) + b * a.z_b + g_base + c_base + first * a.z_t;
+    const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + first * a.B_t;
+    const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + first * a.C_t;
+    const int cols = p.group_channels - c_base;
+    auto fill = [&](int t0) {
+        typename Tl::Raw& r = sh.raw[(t0 - first) / TT & 1];
+        const int rows = len - t0;
+        fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+        fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+        if (!ENDS) {
+            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+        }
+        copy_commit();
+        u_p += TT * a.u_t;
+        d_p += TT * a.delta_t;
+        z_p += TT * a.z_t;
+        B_p += TT * a.B_t;
+        C_p += TT * a.C_t;
+    };
+    if (first < len) fill(first);                               // in flight while the states are set up
+
+    // recurrence role: states n0 .. n0 + S - 1 of channels cl + c * CL of the block
+    const int sl = lane / CL, cl = warp * CW + lane % CL, n0 = sl * S;
+    const long long row = ((long long)b * a.channels + g_base + c_base + cl) * a.states + n0;
+    const long long crow = (long long)CL * a.states;            // from one channel of a lane to the next
+    // a lane's states are one 16-byte access everywhere
+    const bool whole = S == 4 && a.states % 4 == 0
+                       && ((reinterpret_cast<uintptr_t>(a.kept) | reinterpret_cast<uintptr_t>(a.h_last)) & 15) == 0;
+    float2 A2[C][S / 2] = {}, h[C][S / 2] = {};
+    auto cl_ok = [&](int c) { return c_base + cl + c * CL < p.group_channels; };
+    auto get = [&](const float* q, float2(&v)[C][S / 2]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                const float f = q && cl_ok(c) && n0 + s < a.states ? q[c * crow + s] : 0.0f;
+                (s % 2 ? v[c][s / 2].y : v[c][s / 2].x) = f;
+            }
     };
     auto put = [&](float* q) {
-        if (!cl_ok || n0 >= a.states) return;
-        if (whole) {
-            *reinterpret_cast<float4*>(q) = make_float4(h[0].x, h[0].y, h[1].x, h[1].y);
-        } else {
-            const float f[S] = {h[0].x, h[0].y, h[1].x, h[1].y};
 #pragma unroll
-            for (int s = 0; s < S; ++s)
-                if (n0 + s < a.states) q[s] = f[s];
+        for (int c = 0; c < C; ++c) {
+            if (!cl_ok(c) || n0 >= a.states) continue;
+            if (S == 4 && whole) {
+                *reinterpret_cast<float4*>(q + c * crow) =
+                    make_float4(h[c][0].x, h[c][0].y, h[c][S / 2 - 1].x, h[c][S / 2 - 1].y);
+            } else {
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    if (n0 + s < a.states) q[c * crow + s] = s % 2 ? h[c][s / 2].y : h[c][s / 2].x;
+            }
         }
     };
     get(a.A + (g_base + c_base + cl) * a.states + n0, A2);
 #pragma unroll
-    for (int j = 0; j < S / 2; ++j) A2[j] = make_float2(A2[j].x * kLog2e, A2[j].y * kLog2e);
-    if (!ENDS && first < whole_len) {
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < S / 2; ++j) A2[c][j] = make_float2(A2[c][j].x * kLog2e, A2[c][j].y * kLog2e);
+    if constexpr (ENDS) {
+    } else if (first < whole_len) {
         get(a.h0 ? a.h0 + row : nullptr, h);
         const long long rows = a.batch * a.channels;
-        for (int k = 0; k < split; ++k) {
-            float2 end[S / 2];
+        for (int k = 0; k != split; ++k) {
+            float2 end[C][S / 2] = {};
             get(p.ends + k * rows * a.states + row, end);
-            const float d = cl_ok ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl] : 0.0f;
 #pragma unroll
-            for (int j = 0; j < S / 2; ++j)
-                h[j] = make_float2(fmaf(exp2_approx(d * A2[j].x), h[j].x, end[j].x),
-                                   fmaf(exp2_approx(d * A2[j].y), h[j].y, end[j].y));
+            for (int c = 0; c < C; ++c) {
+                const float d = cl_ok(c) ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
+#pragma unroll
+                for (int j = 0; j < S / 2; ++j)
+                    h[c][j] = make_float2(fmaf(exp2_approx(d * A2[c][j].x), h[c][j].x, end[c][j].x),
+                                          fmaf(exp2_approx(d * A2[c][j].y), h[c][j].y, end[c][j].y));
+            }
         }
-    } else if (!ENDS && split == 0) {
+    } else if (split == 0) {
         get(a.h0 ? a.h0 + row : nullptr, h);                    // an empty sequence keeps its state
     }
-    float steps = 0.0f;                                         // sum of d
+    float steps[C] = {};                                        // sums of d
 
-    float u_r[E], d_r[E], z_r[E], B_r[F], C_r[F];
-    auto load = [&](int t0) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const bool ok = ch_ok && t0 + t_e + e * TS < len;
-            u_r[e] = ok ? to_f(*u_p) : 0.0f;
-            d_r[e] = ok ? to_f(*d_p) : 0.0f;
-            u_p += TS * a.u_t;
-            d_p += TS * a.delta_t;
-            if (!ENDS) {
-                z_r[e] = ok && a.z ? to_f(*z_p) : 0.0f;
-                z_p += TS * a.z_t;
-            }
-        }
-#pragma unroll
-        for (int f = 0; f < F; ++f) {
-            const bool ok = t_f + f * DF < TT && n_f < a.states && t0 + t_f + f * DF < len;
-            B_r[f] = ok ? to_f(B_p[f * DF * a.B_t]) : 0.0f;
-            if (!ENDS) C_r[f] = ok ? to_f(C_p[f * DF * a.C_t]) : 0.0f;
-        }
-        B_p += TT * a.B_t;
-        C_p += TT * a.C_t;
-    };
-
-    load(first);
     for (int t0 = first; t0 < len; t0 += TT) {
-        float u_c[E], z_c[E];
+        const typename Tl::Raw& raw = sh.raw[(t0 - first) / TT & 1];
+        copy_wait_all();
+        __syncthreads();
+        if (t0 + TT < len) fill(t0 + TT);
+        if (t_e < TT) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            u_c[e] = u_r[e];
-            if (!ENDS) z_c[e] = z_r[e];
-            const int t = t_e + e * TS;
-            float dt = d_r[e] + bias;
-            if (a.softplus) dt = softplus_f(dt);
-            if (t0 + t >= len) dt = 0.0f;       // a step behind the end leaves the state alone
-            const float du = dt * u_r[e];
-            if (t < TT) sh.d[ch][t] = make_float4(dt, dt, du, du);
+            for (int e = 0; e < E; ++e) {
+                const int t = t_e + e * TS;
+                const Elem u = *reinterpret_cast<const Elem*>(&raw.u[t][ch]);
+                const Elem d = *reinterpret_cast<const Elem*>(&raw.d[t][ch]);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float dt = to_f(d.v[v]) + bias[v];
+                    if (a.softplus) dt = softplus_f(dt);
+                    if (t0 + t >= len) dt = 0.0f;   // a step behind the end leaves the state alone
+                    sh.d[ch + v][t] = make_float2(dt, dt * to_f(u.v[v]));
+                }
+            }
         }
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-            if (t_f + f * DF < TT) {
-                sh.B[t_f + f * DF][n_f] = B_r[f];
-                if (!ENDS) sh.C[t_f + f * DF][n_f] = C_r[f];
-            }
+        for (int i = tid; i < TT * NS; i += NT) {
+            sh.B[0][i] = to_f(raw.B[0][i]);
+            if (!ENDS) sh.C_[0][i] = to_f(raw.C_[0][i]);
         }
         __syncthreads();
-        if (t0 + TT < len) load(t0 + TT);
         if (!ENDS && a.kept && t0 > 0)
             put(a.kept + (long long)(t0 / TT - 1) * a.batch * a.channels * a.states + row);
         // decays that stay near 1 for the whole tile take the polynomial
-        float most = 0.0f;
+        bool near1[C][S];
 #pragma unroll
-        for (int t = 0; t < TT; ++t) most = fmaxf(most, fabsf(sh.d[cl][t].x));
-        bool near1[S];
+        for (int c = 0; c < C; ++c) {
+            float most = 0.0f;
 #pragma unroll
-        for (int j = 0; j < S / 2; ++j) {
-            near1[2 * j] = most * fabsf(A2[j].x) < kExp2Near;
-            near1[2 * j + 1] = most * fabsf(A2[j].y) < kExp2Near;
-        }
-        float y[TT];
+            for (int t = 0; t < TT; t += SL)
+                if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d[cl + c * CL][t + (SL <= TT ? sl : sl % TT)].x));
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const float4 d = sh.d[cl][t];
-            const float4 B4 = *reinterpret_cast<const float4*>(&sh.B[t][n0]);
-            const float4 C4 = ENDS ? B4 : *reinterpret_cast<const float4*>(&sh.C[t][n0]);
-            const float2 dt = make_float2(d.x, d.y), du = make_float2(d.z, d.w);
-            const float2 Bv[2] = {make_float2(B4.x, B4.y), make_float2(B4.z, B4.w)};
-            const float2 Cv[2] = {make_float2(C4.x, C4.y), make_float2(C4.z, C4.w)};
-            float2 acc;
-            if (ENDS) steps += d.x;
+            for (int m = SL / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m * CL));
 #pragma unroll
             for (int j = 0; j < S / 2; ++j) {
-                const float2 x = __fmul2_rn(dt, A2[j]), q = exp2_near1(x);
-                const float2 dec = make_float2(near1[2 * j] ? q.x : exp2_approx(x.x),
-                                               near1[2 * j + 1] ? q.y : exp2_approx(x.y));
-                h[j] = __ffma2_rn(dec, h[j], __fmul2_rn(du, Bv[j]));
-                acc = j == 0 ? __fmul2_rn(h[j], Cv[j]) : __ffma2_rn(h[j], Cv[j], acc);
+                near1[c][2 * j] = most * fabsf(A2[c][j].x) < kExp2Near;
+                near1[c][2 * j + 1] = most * fabsf(A2[c][j].y) < kExp2Near;
             }
-            y[t] = acc.x + acc.y;
         }
-        if (ENDS) {
-            __syncthreads();
-            continue;
-        }
-        using Sums = LaneSums<TT, SL, 1>;
-        Sums::run(y, sl);
-        if (Sums::stores(sl)) {
+        constexpr int R = 8;                    // steps whose sums over the lanes are formed together
 #pragma unroll
-            for (int i = 0; i < Sums::kHeld; ++i) sh.o[cl][Sums::first(sl) + i] = y[i];
+        for (int tr = 0; tr < TT; tr += R) {
+            float y[C][R];
+#pragma unroll
+            for (int t = 0; t < R; ++t) {
+                float2 Bv[S / 2], Cv[S / 2];
+                if constexpr (S == 4) {
+                    const float4 B4 = *reinterpret_cast<const float4*>(&sh.B[tr + t][n0]);
+                    const float4 C4 = ENDS ? B4 : *reinterpret_cast<const float4*>(&sh.C_[tr + t][n0]);
+                    Bv[0] = make_float2(B4.x, B4.y);
+                    Bv[1] = make_float2(B4.z, B4.w);
+                    Cv[0] = make_float2(C4.x, C4.y);
+                    Cv[1] = make_float2(C4.z, C4.w);
+                } else {
+                    Bv[0] = *reinterpret_cast<const float2*>(&sh.B[tr + t][n0]);
+                    Cv[0] = ENDS ? Bv[0] : *reinterpret_cast<const float2*>(&sh.C_[tr + t][n0]);
+                }
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float2 d = sh.d[cl + c * CL][tr + t];
+                    const float2 dt = make_float2(d.x, d.x), du = make_float2(d.y, d.y);
+                    float2 acc;
+                    if (ENDS) steps[c] += d.x;
+#pragma unroll
+                    for (int j = 0; j < S / 2; ++j) {
+                        const float2 x = __fmul2_rn(dt, A2[c][j]), q = exp2_near1(x);
+                        const float2 dec = make_float2(near1[c][2 * j] ? q.x : exp2_approx(x.x),
+                                                       near1[c][2 * j + 1] ? q.y : exp2_approx(x.y));
+                        h[c][j] = __ffma2_rn(dec, h[c][j], __fmul2_rn(du, Bv[j]));
+                        acc = j == 0 ? __fmul2_rn(h[c][j], Cv[j]) : __ffma2_rn(h[c][j], Cv[j], acc);
+                    }
+                    y[c][t] = acc.x + acc.y;
+                }
+            }
+            if (!ENDS) {
+                using Sums = LaneSums<R, SL, CL>;
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    Sums::run(y[c], sl);
+                    if (Sums::stores(sl)) {
+#pragma unroll
+                        for (int i = 0; i < Sums::kHeld; ++i) sh.o[cl + c * CL][tr + Sums::first(sl) + i] = y[c][i];
+                    }
+                }
+            }
         }
+        if (ENDS) continue;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int t = t_e + e * TS;
             if (ch_ok && t0 + t < stop) {
-                float o = fmaf(skip, u_c[e], sh.o[ch][t]);
-                if (a.z) o *= z_c[e] * sigmoid_f(z_c[e]);
-                if (t0 + t >= len) o = 0.0f;
-                *y_p = from_f<IO>(o);
+                const Elem u = *reinterpret_cast<const Elem*>(&raw.u[t][ch]);
+                const Elem z = *reinterpret_cast<const Elem*>(&raw.z[t][ch]);
+                Elem out;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    float o = fmaf(skip[v], to_f(u.v[v]), sh.o[ch + v][t]);
+                    if (a.z) o *= to_f(z.v[v]) * sigmoid_f(to_f(z.v[v]));
+                    if (t0 + t >= len) o = 0.0f;
+                    out.v[v] = from_f<IO>(o);
+                }
+                *reinterpret_cast<Elem*>(y_p) = out;
             }
             y_p += TS * a.y_t;
         }
     }
     if (ENDS) {
         put(p.ends + split * a.batch * a.channels * a.states + row);
-        if (cl_ok && sl == 0)
-            p.end_steps[(split * a.batch + b) * a.channels + g_base + c_base + cl] = steps;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+            if (cl_ok(c) && sl == 0)
+                p.end_steps[(split * a.batch + b) * a.channels + g_base + c_base + cl + c * CL] = steps[c];
         return;
     }
     // rows behind the end (y_p is at the tile behind the last)
     if (ch_ok) {
+        Elem none;
+#pragma unroll
+        for (int v = 0; v < V; ++v) none.v[v] = from_f<IO>(0.0f);
         const int done = len > first ? first + (len - first + TT - 1) / TT * TT : first;
-        for (long long t = done + t_e; t < stop; t += TS, y_p += TS * a.y_t) *y_p = from_f<IO>(0.0f);
+        for (long long t = done + t_e; t < stop; t += TS, y_p += TS * a.y_t)
+            *reinterpret_cast<Elem*>(y_p) = none;
     }
     if (a.h_last && (first < whole_len ? whole_len <= stop : split == 0 && whole_len == 0)) put(a.h_last + row);
 }
 
-template <typename IO, int SL>
+template <typename IO, int S, int SL, int C, bool WIDE>
+cudaError_t launch_form(const ScanParams& p, unsigned blocks, cudaStream_t st) {
+    constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
+    if (smem > 48 * 1024) {
+        cudaError_t e = cudaFuncSetAttribute(scan_fwd<IO, S, SL, C, WIDE, true>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(scan_fwd<IO, S, SL, C, WIDE, false>,
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    if (p.splits > 1)
+        scan_fwd<IO, S, SL, C, WIDE, true><<<blocks * (p.splits - 1), NT, smem, st>>>(p);
+    scan_fwd<IO, S, SL, C, WIDE, false><<<blocks * p.splits, NT, smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename IO, int S, int SL, int C>
 cudaError_t launch(ScanParams p, cudaStream_t st) {
-    constexpr int BC = Tile<SL>::BC;
+    constexpr int BC = Tile<IO, S, SL, C>::BC;
     p.tiles = (p.group_channels + BC - 1) / BC;
     const long long blocks = (long long)p.tiles * p.a.groups * p.a.batch;
     if (blocks > 0x7fffffffLL / p.splits) return cudaErrorInvalidValue;
-    if (p.splits > 1)
-        scan_fwd<IO, SL, true><<<(unsigned)(blocks * (p.splits - 1)), NT, sizeof(Tile<SL>), st>>>(p);
-    scan_fwd<IO, SL, false><<<(unsigned)(blocks * p.splits), NT, sizeof(Tile<SL>), st>>>(p);
-    return cudaGetLastError();
+    const dfsnn_state_scan_args& a = p.a;
+    p.words = rows_aligned(p, sizeof(IO), 4);
+    const bool pairs = p.group_channels % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % (2 * sizeof(IO)) == 0 && a.y_t % 2 == 0 && a.y_b % 2 == 0;
+    return pairs && rows_aligned(p, sizeof(IO), 16) ? launch_form<IO, S, SL, C, true>(p, (unsigned)blocks, st)
+                                                    : launch_form<IO, S, SL, C, false>(p, (unsigned)blocks, st);
 }
 
 template <typename IO>
 cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     const int n = p.a.states;
-    if (n <= 4) return launch<IO, 1>(p, st);
-    if (n <= 8) return launch<IO, 2>(p, st);
-    if (n <= 16) return launch<IO, 4>(p, st);
-    if (n <= 32) return launch<IO, 8>(p, st);
-    if (n <= 64) return launch<IO, 16>(p, st);
-    return launch<IO, 32>(p, st);
+    if (n <= 4) return launch<IO, 2, 2, 1>(p, st);
+    if (n <= 8) return launch<IO, 2, 4, 1>(p, st);
+    if (n <= 16) return launch<IO, 4, 4, 1>(p, st);
+    if (n <= 32) return launch<IO, 4, 8, 1>(p, st);
+    if (n <= 64) return launch<IO, 4, 16, 1>(p, st);
+    return launch<IO, 4, 32, 1>(p, st);
 }
 
-// Channels of a block
+// Channels of a block, as pick() has them
 int block_channels(int states) {
-    int sl = 1;
-    while (sl * S < states) sl *= 2;
-    return NT / 32 * (32 / sl);
+    if (states <= 4) return Tile<float, 2, 2, 1>::BC;
+    if (states <= 8) return Tile<float, 2, 4, 1>::BC;
+    if (states <= 16) return Tile<float, 4, 4, 1>::BC;
+    if (states <= 32) return Tile<float, 4, 8, 1>::BC;
+    if (states <= 64) return Tile<float, 4, 16, 1>::BC;
+    return Tile<float, 4, 32, 1>::BC;
 }
 
 }  // namespace

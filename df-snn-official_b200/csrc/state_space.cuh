@@ -30,8 +30,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+// 1 / x by the hardware approximation (1 ulp); x = inf gives 0
+__device__ __forceinline__ float rcp_ftz(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ float sigmoid_f(float x) {
-    return __fdividef(1.0f, 1.0f + exp2_approx(-kLog2e * x));
+    return rcp_ftz(1.0f + exp2_approx(-kLog2e * x));
 }
 
 // log(1 + e^x) = max(x, 0) + log(1 + v), v = e^-|x|, which loses nothing at either end.  The
@@ -39,7 +46,7 @@ __device__ __forceinline__ float sigmoid_f(float x) {
 // fitted at Chebyshev nodes in s^2 (0.07 units of 2^-24 off), in a third of log1pf's instructions.
 __device__ __forceinline__ float softplus_f(float x) {
     const float v = exp2_approx(-kLog2e * fabsf(x));
-    const float s = __fdividef(v, 2.0f + v), w = s * s;
+    const float s = v * rcp_ftz(2.0f + v), w = s * s;
     float q = fmaf(w, 0.2817465727f, 0.2796141883f);
     q = fmaf(w, q, 0.4002485372f);
     q = fmaf(w, q, 0.6666631594f);

@@ -118,6 +118,20 @@ def test_scan_batch_first_views():
     assert torch.autograd.grad(y.float().sum(), u)[0].shape == u.shape
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shift", [0, 1, 2, 4])
+@pytest.mark.parametrize("D,N,G", [(64, 16, 1), (66, 12, 2), (33, 7, 1), (24, 100, 1), (8, 3, 1)])
+def test_scan_alignments(D, N, G, shift, dtype):
+    """Rows that start on 16 bytes, on 4 and on less, widths that end inside a 16-byte piece."""
+    x, n, grads = scan_case(21, 2, D, N, G, dtype, lengths=[21, 18], seed=D + shift)
+    for k in ("u", "delta", "z", "B", "C"):
+        v = x[k].flatten(2)
+        w = torch.empty(*v.shape[:2], v.shape[2] + 8, dtype=v.dtype, device=DEV).fill_(float("nan"))
+        w[..., shift:shift + v.shape[2]] = v
+        x[k] = w[..., shift:shift + v.shape[2]].unflatten(2, x[k].shape[2:])
+    check_scan(x, n, grads, True, f"shift {shift}")
+
+
 @pytest.mark.parametrize("T,B,D,N,G,lengths", [
     (1000, 1, 40, 16, 1, None), (2049, 4, 36, 16, 2, [2049, 700, 0, 1]), (1500, 2, 12, 100, 1, [16, 1024]),
     (999, 1, 130, 3, 1, None), (1040, 3, 9, 33, 3, [1040, 1039, 129])])
