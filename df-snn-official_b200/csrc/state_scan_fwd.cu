@@ -38,11 +38,26 @@ struct Tile {
     struct Raw {                                       // as the sequences have them
         IO u[TT][BC], d[TT][BC], z[TT][BC], B[TT][NS], C_[TT][NS];
     };
+    template <int K> using Pieces = TilePieces<IO, TT, NT, K>;
+    template <int COLS> static constexpr int kPieces = Pieces<1>::template kPieces<COLS>;
+    static constexpr bool kEights = BC * sizeof(IO) < 16 || NS * sizeof(IO) < 16;   // rows of 8 bytes
     __align__(16) Raw raw[2];                          // this tile's and the next one's
     float2 d[BC][TT + 1];                              // (d, d u)
     __align__(16) float B[TT][NS], C_[TT][NS];
     float o[BC][TT + 1];
 };
+
+// S neighbouring states as pairs
+template <int S>
+__device__ __forceinline__ void load_states(float2 (&v)[S / 2], const float* q) {
+    if constexpr (S == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(q);
+        v[0] = make_float2(f.x, f.y);
+        v[1] = make_float2(f.z, f.w);
+    } else {
+        v[0] = *reinterpret_cast<const float2*>(q);
+    }
+}
 
 // V neighbouring elements of a sequence
 template <typename IO, int V>
@@ -98,22 +113,39 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
     const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + first * a.B_t;
     const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + first * a.C_t;
     const int cols = p.group_channels - c_base;
-    auto fill = [&](int t0) {
-        typename Tl::Raw& r = sh.raw[(t0 - first) / TT & 1];
-        const int rows = len - t0;
-        fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words);
-        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
-        fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+    using Raw = typename Tl::Raw;
+    Raw& raw0 = sh.raw[0];
+    constexpr int K = ((ENDS ? 2 : 3) * Tl::template kPieces<BC> + (ENDS ? 1 : 2) * Tl::template kPieces<NS> + NT - 1) / NT;
+    typename Tl::template Pieces<WIDE ? K : 1> pieces;
+    if constexpr (WIDE) {
+        pieces.template add<BC>(raw0.u, u_p, a.u_t, cols);
+        pieces.template add<BC>(raw0.d, d_p, a.delta_t, cols);
+        pieces.template add<NS>(raw0.B, B_p, a.B_t, a.states);
         if (!ENDS) {
-            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words);
-            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+            pieces.template add<NS>(raw0.C_, C_p, a.C_t, a.states);
+            if (a.z) pieces.template add<BC>(raw0.z, z_p, a.z_t, cols);
+        }
+    }
+    auto fill = [&](int t0) {
+        const int stage = (t0 - first) / TT & 1, rows = len - t0;
+        if constexpr (WIDE) {
+            pieces.template issue<Tl::kEights>(stage * (unsigned)sizeof(Raw), rows);
+        } else {
+            Raw& r = sh.raw[stage];
+            fill_tile<IO, TT, BC, NT>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+            if (!ENDS) {
+                if (a.z) fill_tile<IO, TT, BC, NT>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+                fill_tile<IO, TT, NS, NT>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+            }
+            u_p += TT * a.u_t;
+            d_p += TT * a.delta_t;
+            z_p += TT * a.z_t;
+            B_p += TT * a.B_t;
+            C_p += TT * a.C_t;
         }
         copy_commit();
-        u_p += TT * a.u_t;
-        d_p += TT * a.delta_t;
-        z_p += TT * a.z_t;
-        B_p += TT * a.B_t;
-        C_p += TT * a.C_t;
     };
     if (first < len) fill(first);                               // in flight while the states are set up
 
@@ -176,7 +208,7 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
     float steps[C] = {};                                        // sums of d
 
     for (int t0 = first; t0 < len; t0 += TT) {
-        const typename Tl::Raw& raw = sh.raw[(t0 - first) / TT & 1];
+        const Raw& raw = sh.raw[(t0 - first) / TT & 1];
         copy_wait_all();
         __syncthreads();
         if (t0 + TT < len) fill(t0 + TT);
@@ -186,12 +218,13 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
                 const int t = t_e + e * TS;
                 const Elem u = *reinterpret_cast<const Elem*>(&raw.u[t][ch]);
                 const Elem d = *reinterpret_cast<const Elem*>(&raw.d[t][ch]);
+                float2 dt = make_float2(to_f(d.v[0]) + bias[0], to_f(d.v[V - 1]) + bias[V - 1]);
+                if (a.softplus) dt = softplus_f(dt);
+                if (t0 + t >= len) dt = make_float2(0.0f, 0.0f);    // a step behind the end leaves the state alone
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    float dt = to_f(d.v[v]) + bias[v];
-                    if (a.softplus) dt = softplus_f(dt);
-                    if (t0 + t >= len) dt = 0.0f;   // a step behind the end leaves the state alone
-                    sh.d[ch + v][t] = make_float2(dt, dt * to_f(u.v[v]));
+                    const float x = v ? dt.y : dt.x;
+                    sh.d[ch + v][t] = make_float2(x, x * to_f(u.v[v]));
                 }
             }
         }
@@ -223,35 +256,42 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
 #pragma unroll
         for (int tr = 0; tr < TT; tr += R) {
             float y[C][R];
+            constexpr int G = 4;                // steps whose decays are formed before their states
 #pragma unroll
-            for (int t = 0; t < R; ++t) {
-                float2 Bv[S / 2], Cv[S / 2];
-                if constexpr (S == 4) {
-                    const float4 B4 = *reinterpret_cast<const float4*>(&sh.B[tr + t][n0]);
-                    const float4 C4 = ENDS ? B4 : *reinterpret_cast<const float4*>(&sh.C_[tr + t][n0]);
-                    Bv[0] = make_float2(B4.x, B4.y);
-                    Bv[1] = make_float2(B4.z, B4.w);
-                    Cv[0] = make_float2(C4.x, C4.y);
-                    Cv[1] = make_float2(C4.z, C4.w);
-                } else {
-                    Bv[0] = *reinterpret_cast<const float2*>(&sh.B[tr + t][n0]);
-                    Cv[0] = ENDS ? Bv[0] : *reinterpret_cast<const float2*>(&sh.C_[tr + t][n0]);
+            for (int tg = 0; tg < R; tg += G) {
+                float2 dec[G][C][S / 2], in[G][C][S / 2];
+#pragma unroll
+                for (int t = 0; t < G; ++t) {
+                    float2 Bv[S / 2];
+                    load_states<S>(Bv, &sh.B[tr + tg + t][n0]);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) {
+                        const float2 d = sh.d[cl + c * CL][tr + tg + t];
+                        const float2 dt = make_float2(d.x, d.x), du = make_float2(d.y, d.y);
+                        if (ENDS) steps[c] += d.x;
+#pragma unroll
+                        for (int j = 0; j < S / 2; ++j) {
+                            const float2 x = __fmul2_rn(dt, A2[c][j]), q = exp2_near1(x);
+                            dec[t][c][j] = make_float2(near1[c][2 * j] ? q.x : exp2_approx(x.x),
+                                                       near1[c][2 * j + 1] ? q.y : exp2_approx(x.y));
+                            in[t][c][j] = __fmul2_rn(du, Bv[j]);
+                        }
+                    }
                 }
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const float2 d = sh.d[cl + c * CL][tr + t];
-                    const float2 dt = make_float2(d.x, d.x), du = make_float2(d.y, d.y);
-                    float2 acc;
-                    if (ENDS) steps[c] += d.x;
+                for (int t = 0; t < G; ++t) {
+                    float2 Cv[S / 2];
+                    if (!ENDS) load_states<S>(Cv, &sh.C_[tr + tg + t][n0]);
 #pragma unroll
-                    for (int j = 0; j < S / 2; ++j) {
-                        const float2 x = __fmul2_rn(dt, A2[c][j]), q = exp2_near1(x);
-                        const float2 dec = make_float2(near1[c][2 * j] ? q.x : exp2_approx(x.x),
-                                                       near1[c][2 * j + 1] ? q.y : exp2_approx(x.y));
-                        h[c][j] = __ffma2_rn(dec, h[c][j], __fmul2_rn(du, Bv[j]));
-                        acc = j == 0 ? __fmul2_rn(h[c][j], Cv[j]) : __ffma2_rn(h[c][j], Cv[j], acc);
+                    for (int c = 0; c < C; ++c) {
+                        float2 acc;
+#pragma unroll
+                        for (int j = 0; j < S / 2; ++j) {
+                            h[c][j] = __ffma2_rn(dec[t][c][j], h[c][j], in[t][c][j]);
+                            if (!ENDS) acc = j == 0 ? __fmul2_rn(h[c][j], Cv[j]) : __ffma2_rn(h[c][j], Cv[j], acc);
+                        }
+                        if (!ENDS) y[c][tg + t] = acc.x + acc.y;
                     }
-                    y[c][t] = acc.x + acc.y;
                 }
             }
             if (!ENDS) {
@@ -274,14 +314,16 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
             if (ch_ok && t0 + t < stop) {
                 const Elem u = *reinterpret_cast<const Elem*>(&raw.u[t][ch]);
                 const Elem z = *reinterpret_cast<const Elem*>(&raw.z[t][ch]);
-                Elem out;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    float o = fmaf(skip[v], to_f(u.v[v]), sh.o[ch + v][t]);
-                    if (a.z) o *= to_f(z.v[v]) * sigmoid_f(to_f(z.v[v]));
-                    if (t0 + t >= len) o = 0.0f;
-                    out.v[v] = from_f<IO>(o);
+                float2 o = make_float2(fmaf(skip[0], to_f(u.v[0]), sh.o[ch][t]),
+                                       fmaf(skip[V - 1], to_f(u.v[V - 1]), sh.o[ch + V - 1][t]));
+                if (a.z) {
+                    const float2 zf = make_float2(to_f(z.v[0]), to_f(z.v[V - 1]));
+                    o = __fmul2_rn(o, __fmul2_rn(zf, sigmoid_f(zf)));
                 }
+                if (t0 + t >= len) o = make_float2(0.0f, 0.0f);
+                Elem out;
+                out.v[0] = from_f<IO>(o.x);
+                out.v[V - 1] = from_f<IO>(V == 1 ? o.x : o.y);
                 *reinterpret_cast<Elem*>(y_p) = out;
             }
             y_p += TS * a.y_t;

@@ -41,18 +41,27 @@ __device__ __forceinline__ float sigmoid_f(float x) {
     return rcp_ftz(1.0f + exp2_approx(-kLog2e * x));
 }
 
+__device__ __forceinline__ float2 sigmoid_f(float2 x) {
+    const float2 y = __fmul2_rn(x, make_float2(-kLog2e, -kLog2e));
+    const float2 d = __fadd2_rn(make_float2(exp2_approx(y.x), exp2_approx(y.y)), make_float2(1.0f, 1.0f));
+    return make_float2(rcp_ftz(d.x), rcp_ftz(d.y));
+}
+
 // log(1 + e^x) = max(x, 0) + log(1 + v), v = e^-|x|, which loses nothing at either end.  The
 // logarithm by its series log(1 + v) = 2 atanh(s), s = v / (2 + v) <= 1/3: an odd polynomial in s,
 // fitted at Chebyshev nodes in s^2 (0.07 units of 2^-24 off), in a third of log1pf's instructions.
-__device__ __forceinline__ float softplus_f(float x) {
-    const float v = exp2_approx(-kLog2e * fabsf(x));
-    const float s = v * rcp_ftz(2.0f + v), w = s * s;
-    float q = fmaf(w, 0.2817465727f, 0.2796141883f);
-    q = fmaf(w, q, 0.4002485372f);
-    q = fmaf(w, q, 0.6666631594f);
-    q = fmaf(w, q, 2.0f);
-    return fmaf(s, q, fmaxf(x, 0.0f));
+__device__ __forceinline__ float2 softplus_f(float2 x) {
+    auto two = [](float c) { return make_float2(c, c); };
+    const float2 v = make_float2(exp2_approx(-kLog2e * fabsf(x.x)), exp2_approx(-kLog2e * fabsf(x.y)));
+    const float2 d = __fadd2_rn(v, two(2.0f));
+    const float2 s = __fmul2_rn(v, make_float2(rcp_ftz(d.x), rcp_ftz(d.y))), w = __fmul2_rn(s, s);
+    float2 q = __ffma2_rn(w, two(0.2817465727f), two(0.2796141883f));
+    q = __ffma2_rn(w, q, two(0.4002485372f));
+    q = __ffma2_rn(w, q, two(0.6666631594f));
+    q = __ffma2_rn(w, q, two(2.0f));
+    return __ffma2_rn(s, q, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
 }
+__device__ __forceinline__ float softplus_f(float x) { return softplus_f(make_float2(x, x)).x; }
 
 // 2^x for |x| < 2^-4, two at a time: 1 + x p(x), fitted at Chebyshev nodes (0.64 units of 2^-24
 // off).  Near 1 the hardware's approximation is off by up to 2^-22, and a state that decays by
