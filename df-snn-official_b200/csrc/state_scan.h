@@ -4,9 +4,8 @@
 
 namespace dfsnn {
 
-constexpr int kScanChunk = DFSNN_SCAN_CHUNK;   // steps of a tile
-constexpr int kScanPitch = kScanChunk + 4;     // floats of a row in shared memory: 16-byte rows,
-                                               // eight of which start on different banks
+constexpr int kScanTile = 16;                  // steps of a tile
+constexpr int kScanChunk = DFSNN_SCAN_CHUNK;   // steps between kept states
 
 struct ScanParams {
     dfsnn_state_scan_args a;
@@ -25,17 +24,22 @@ struct ScanParams {
     float* part_d;                             // [2][batch_parts][channels] (D, delta_bias)
 };
 
-// Whether every row (a step's channels of a group, a step's states) of the forward's inputs starts
-// on a multiple of `bytes`.  Channel tiles start on multiples of 4 channels, whole rows of a tile.
+// Whether every row (a step's channels of a group, a step's states) of the inputs starts on a
+// multiple of `bytes`.  Channel tiles start on multiples of 4 channels, whole rows of a tile.
 inline bool rows_aligned(const ScanParams& p, size_t elem, size_t bytes) {
     const dfsnn_state_scan_args& a = p.a;
     auto ok = [&](const void* q, long long t, long long b, long long g) {
         return reinterpret_cast<uintptr_t>(q) % bytes == 0 && t * (long long)elem % (long long)bytes == 0
                && b * (long long)elem % (long long)bytes == 0 && g * (long long)elem % (long long)bytes == 0;
     };
-    const long long gc = p.group_channels;
-    return ok(a.u, a.u_t, a.u_b, a.groups > 1 ? gc : 0) && ok(a.delta, a.delta_t, a.delta_b, 0)
-           && ok(a.z, a.z_t, a.z_b, 0) && ok(a.B, a.B_t, a.B_b, a.B_g) && ok(a.C, a.C_t, a.C_b, a.C_g);
+    return ok(a.u, a.u_t, a.u_b, a.groups > 1 ? p.group_channels : 0) && ok(a.delta, a.delta_t, a.delta_b, 0)
+           && ok(a.z, a.z_t, a.z_b, 0) && ok(a.B, a.B_t, a.B_b, a.B_g) && ok(a.C, a.C_t, a.C_b, a.C_g)
+           && ok(p.g.grad_y, a.y_t, a.y_b, 0);
+}
+
+// Whether pairs of neighbouring channels of an output start on a multiple of two elements
+inline bool pairs_aligned(const void* q, long long t, long long b, size_t elem) {
+    return reinterpret_cast<uintptr_t>(q) % (2 * elem) == 0 && t % 2 == 0 && b % 2 == 0;
 }
 
 int state_scan_splits(long long T, long long batch, long long group_channels, int groups, int states);

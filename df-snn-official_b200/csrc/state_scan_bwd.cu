@@ -4,49 +4,91 @@
 //   l_t = C_t g_t + a_(t+1) l_(t+1),   a_t = exp(d_t A),   q_t = a_t l_t h_(t-1)
 //   grad C_t = sum_c g_t h_t     grad B_t = sum_c l_t d_t u_t     grad A = sum_(t,b) q_t d_t
 //   grad u_t = d_t sum_n l_t B_t + D g_t      grad d_t = u_t sum_n l_t B_t + sum_n q_t A
-// A warp walks the sequence of its channels backwards in chunks of 16 steps.  The forward kept
-// the state in front of every chunk; from it the chunk's states and decays are formed again and
-// stay in registers (2 * 16 floats for each state that a lane holds), so each exponential is
-// taken once.  The sums over states (a channel's lanes) and over channels (the other lanes) are
-// formed for several steps at a time (LaneSums).  The sums over channels then go over the warps
-// in shared memory and over the blocks through partial sums that a second kernel adds in a fixed
-// order; no atomics, so results do not change from run to run.
+// A warp walks the sequence of its channels backwards.  The forward kept the state in front of
+// every 8 steps; from it the 8 steps' states and decays are formed again and stay in registers, so
+// each exponential is taken once.  About 12 multiply-adds and one exponential for each (step,
+// channel, state): bound by the issue of instructions.  Hence packed pairs of states; four states
+// and two channels a lane, which halves the shuffles of the two kinds of sums, over states (a
+// channel's SL lanes) and over channels (the other lanes), both formed for 8 steps at a time
+// (LaneSums); elementwise work once per (step, channel) by all threads.  The sums over channels go
+// on over the warps in shared memory and over the blocks through partial sums that a second kernel
+// adds in a fixed order: no atomics, so results do not change from run to run.
 #include <algorithm>
 
 #include "state_scan.h"
+#include "state_tile.cuh"
 
 namespace dfsnn {
 namespace {
 
-constexpr int TT = kScanChunk, P = kScanPitch;
-constexpr int NT = 128;
+constexpr int TT = kScanTile, R = kScanChunk;
+constexpr int Q = 4;                                 // steps whose sums over lanes are formed together
+constexpr int NT = 128, NW = NT / 32;
 
-template <int S, int C, int SL>
-struct Shape {
+// S states on each of a channel's SL lanes, C channels a lane
+template <typename IO, int S, int SL, int C>
+struct Tile {
     static constexpr int CL = 32 / SL;               // channel lanes of a warp
-    static constexpr int NW = NT / 32;
-    static constexpr int BC = NW * CL * C;           // channels of the block
+    static constexpr int CW = CL * C;                // channels of a warp
+    static constexpr int BC = NW * CW;               // channels of the block
     static constexpr int NS = S * SL;                // states, padded
-    static constexpr size_t smem(bool gate) {
-        return sizeof(float) * ((size_t)(gate ? 4 : 3) * BC * P + 2 * (size_t)NS * P
-                                + (size_t)NW * 2 * TT * NS);
-    }
+    struct Raw {                                     // as the sequences have them
+        IO u[TT][BC], d[TT][BC], z[TT][BC], g[TT][BC], B[TT][NS], C_[TT][NS];
+    };
+    __align__(16) Raw raw[2];                        // this tile's and the next one's
+    __align__(16) float B[TT][NS], C_[TT][NS];
+    __align__(16) float red[NW][2][TT][NS];          // the warps' sums over channels (grad B, grad C)
+    float2 d[BC][TT + 1];                            // (d, d u)
+    float g[BC][TT + 1];                             // grad o
+    float lb[BC][TT + 1], qa[BC][TT + 1], o[BC][TT + 1];    // sums over states
+    float sums[2][NT];
 };
 
-template <typename IO, int S, int C, int SL, bool GATE>
-__global__ void __launch_bounds__(NT) scan_bwd(const ScanParams p) {
-    using Sh = Shape<S, C, SL>;
-    constexpr int CL = Sh::CL, NW = Sh::NW, BC = Sh::BC, NS = Sh::NS;
-    constexpr int E = (TT * BC + NT - 1) / NT, TS = TT / E;
-    constexpr int F = (TT * NS + NT - 1) / NT;
-    extern __shared__ __align__(16) float smem[];
-    float(*s_dt)[P] = reinterpret_cast<float(*)[P]>(smem);
-    float(*s_u)[P] = s_dt + BC;
-    float(*s_g)[P] = s_u + BC;
-    float(*s_o)[P] = s_g + BC;                                 // with a gate only
-    float(*s_B)[P] = GATE ? s_o + BC : s_o;
-    float(*s_C)[P] = s_B + NS;
-    float* s_red = reinterpret_cast<float*>(s_C + NS);         // [NW][2][TT][NS]
+template <int S>
+__device__ __forceinline__ void load_states(float2 (&v)[S / 2], const float* q) {
+    if constexpr (S == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(q);
+        v[0] = make_float2(f.x, f.y);
+        v[1] = make_float2(f.z, f.w);
+    } else {
+        v[0] = *reinterpret_cast<const float2*>(q);
+    }
+}
+template <int S, int Q>
+__device__ __forceinline__ void store_states(float* q, const float (&v)[S][Q], int i) {
+    if constexpr (S == 4) *reinterpret_cast<float4*>(q) = make_float4(v[0][i], v[1][i], v[2][i], v[3][i]);
+    else *reinterpret_cast<float2*>(q) = make_float2(v[0][i], v[1][i]);
+}
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+
+// V neighbouring elements of a sequence
+template <typename IO, int V>
+struct __align__(sizeof(IO) * V) Pack {
+    IO v[V];
+};
+template <typename IO, int V>
+__device__ __forceinline__ float2 unpack(const IO* q) {
+    const Pack<IO, V> p = *reinterpret_cast<const Pack<IO, V>*>(q);
+    return make_float2(to_f(p.v[0]), to_f(p.v[V - 1]));
+}
+template <typename IO, int V>
+__device__ __forceinline__ void store(IO* q, float2 f) {
+    Pack<IO, V> p;
+    p.v[0] = from_f<IO>(f.x);
+    if (V == 2) p.v[V - 1] = from_f<IO>(f.y);
+    *reinterpret_cast<Pack<IO, V>*>(q) = p;
+}
+
+template <typename IO, int S, int SL, int C, bool WIDE>
+__global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
+    using Tl = Tile<IO, S, SL, C>;
+    constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS, J = S / 2;
+    constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
+    constexpr int ROW = BC / V;                                 // threads along a step's channels
+    constexpr int E = TT * ROW > NT ? TT * ROW / NT : 1;        // packs of a thread,
+    constexpr int TS = TT / E;                                  // this many steps apart
+    extern __shared__ __align__(16) unsigned char smem[];
+    Tl& sh = *reinterpret_cast<Tl*>(smem);
     const dfsnn_state_scan_args& a = p.a;
     const dfsnn_state_scan_grads& g = p.g;
 
@@ -56,212 +98,252 @@ __global__ void __launch_bounds__(NT) scan_bwd(const ScanParams p) {
     bid /= p.tiles;
     const int grp = (int)(bid % a.groups);
     const int part = (int)(bid / a.groups);
-    const int c_base = tile * BC;
+    const int c_base = tile * BC, cols = p.group_channels - c_base;
     const long long g_base = (long long)grp * p.group_channels;
 
-    // elementwise role: thread's channel ch, steps t_e + e * TS
-    const int ch = tid % BC, t_e = tid / BC;
-    const bool ch_ok = c_base + ch < p.group_channels && t_e < TT;
+    // elementwise role: packs (step t_e + e * TS, channels ch .. ch + V - 1)
+    const int ch = tid % ROW * V, t_e = tid / ROW;
+    const bool ch_ok = ch < cols && t_e < TT;
     const long long chan = g_base + c_base + ch;
-    const float bias = ch_ok && a.delta_bias ? a.delta_bias[chan] : 0.0f;
-    const float skip = ch_ok && a.D ? a.D[chan] : 0.0f;
-    float sum_D = 0.0f, sum_bias = 0.0f;
+    float2 bias = two(0.0f), skip = two(0.0f), sum_D = two(0.0f), sum_bias = two(0.0f);
+    if (ch_ok && a.delta_bias) bias = make_float2(a.delta_bias[chan], a.delta_bias[chan + V - 1]);
+    if (ch_ok && a.D) skip = make_float2(a.D[chan], a.D[chan + V - 1]);
 
-    // recurrence role: states s * SL + sl of channels c * CL + lane / SL of this warp
-    const int sl = lane % SL, cl = lane / SL;
-    float A2[C][S], dA[C][S];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int k = c_base + warp * CL * C + c * CL + cl, n = s * SL + sl;
-            const bool ok = k < p.group_channels && n < a.states;
-            A2[c][s] = ok ? a.A[(g_base + k) * a.states + n] * kLog2e : 0.0f;
-            dA[c][s] = 0.0f;
-        }
-
-    for (long long b = part; b < a.batch; b += p.batch_parts) {
-        const int len = seq_length(a.lengths, a.lengths64, b, p.T);
-        const IO* u_p = static_cast<const IO*>(a.u) + b * a.u_b + chan;
-        const IO* d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + chan;
-        const IO* z_p = GATE ? static_cast<const IO*>(a.z) + b * a.z_b + chan : nullptr;
-        const IO* gy_p = static_cast<const IO*>(g.grad_y) + b * a.y_b + chan;
-        IO* gu_p = static_cast<IO*>(g.grad_u) + b * g.gu_b + chan;
-        IO* gd_p = static_cast<IO*>(g.grad_delta) + b * g.gdelta_b + chan;
-        IO* gz_p = GATE && g.grad_z ? static_cast<IO*>(g.grad_z) + b * g.gz_b + chan : nullptr;
-        const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g;
-        const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g;
-        const long long row0 = ((long long)b * a.channels + g_base + c_base + warp * CL * C + cl) * a.states;
-
-        float lam[C][S];                                       // a_(t+1) l_(t+1)
+    // recurrence role: states n0 .. n0 + S - 1 of channels cl + c * CL of the block
+    const int sl = lane / CL, lc = lane % CL, cl = warp * CW + lc, n0 = sl * S;
+    const long long crow = (long long)CL * a.states;
+    auto get = [&](const float* q, float2(&v)[C][J]) {
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                const int n = s * SL + sl;
-                const bool ok = c_base + warp * CL * C + c * CL + cl < p.group_channels && n < a.states;
-                lam[c][s] = ok && g.grad_h_last ? g.grad_h_last[row0 + (long long)c * CL * a.states + n] : 0.0f;
+                const float f = q && cl + c * CL < cols && n0 + s < a.states ? q[c * crow + s] : 0.0f;
+                (s % 2 ? v[c][s / 2].y : v[c][s / 2].x) = f;
             }
+    };
+    auto put = [&](float* q, const float2(&v)[C][J]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (cl + c * CL < cols && n0 + s < a.states) q[c * crow + s] = s % 2 ? v[c][s / 2].y : v[c][s / 2].x;
+    };
+    float2 A2[C][J] = {}, dA[C][J] = {};
+    get(a.A + (g_base + c_base + cl) * a.states + n0, A2);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < J; ++j) A2[c][j] = __fmul2_rn(A2[c][j], two(kLog2e));
+
+    for (long long b = part; b < a.batch; b += p.batch_parts) {
+        const int len = seq_length(a.lengths, a.lengths64, b, p.T);
+        const int top = len > 0 ? (len - 1) / TT * TT : -1;     // first step of the last tile
+        IO* gu_p = static_cast<IO*>(g.grad_u) + b * g.gu_b + chan + t_e * g.gu_t;
+        IO* gd_p = static_cast<IO*>(g.grad_delta) + b * g.gdelta_b + chan + t_e * g.gdelta_t;
+        IO* gz_p = static_cast<IO*>(g.grad_z) + b * g.gz_b + chan + t_e * g.gz_t;
+        const long long row = ((long long)b * a.channels + g_base + c_base + cl) * a.states + n0;
+
+        // the block's sequences at the last tile
+        const IO* u_p = static_cast<const IO*>(a.u) + b * a.u_b + g_base + c_base + top * a.u_t;
+        const IO* d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + g_base + c_base + top * a.delta_t;
+        const IO* z_p = static_cast<const IO*>(a.z) + b * a.z_b + g_base + c_base + top * a.z_t;
+        const IO* g_p = static_cast<const IO*>(g.grad_y) + b * a.y_b + g_base + c_base + top * a.y_t;
+        const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + top * a.B_t;
+        const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + top * a.C_t;
+        using Raw = typename Tl::Raw;
+        auto fill = [&](int t0) {
+            const int rows = len - t0;
+            Raw& r = sh.raw[t0 / TT & 1];
+            fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], g_p, a.y_t, rows, cols, p.words);
+            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+            u_p -= TT * a.u_t;
+            d_p -= TT * a.delta_t;
+            z_p -= TT * a.z_t;
+            g_p -= TT * a.y_t;
+            B_p -= TT * a.B_t;
+            C_p -= TT * a.C_t;
+            copy_commit();
+        };
+        if (top >= 0) fill(top);
+
+        // the state in front of the 8 steps from t on
+        auto state_at = [&](int t, float2(&v)[C][J]) {
+            get(t > 0 ? a.kept + (long long)(t / R - 1) * a.batch * a.channels * a.states + row
+                      : (a.h0 ? a.h0 + row : nullptr), v);
+        };
+        float2 start[C][J] = {};                                // loaded one chunk ahead
+        if (top >= 0) state_at((len - 1) / R * R, start);
+        float2 lam[C][J] = {};                                  // a_(t+1) l_(t+1)
+        get(g.grad_h_last ? g.grad_h_last + row : nullptr, lam);
 
         // rows behind the end
         if (ch_ok)
-            for (long long t = (long long)(len + TT - 1) / TT * TT + t_e; t < p.T; t += TS) {
-                gu_p[t * g.gu_t] = from_f<IO>(0.0f);
-                gd_p[t * g.gdelta_t] = from_f<IO>(0.0f);
-                if (GATE && gz_p) gz_p[t * g.gz_t] = from_f<IO>(0.0f);
+            for (long long t = (long long)top + (top < 0 ? 1 : TT) + t_e; t < p.T; t += TS) {
+                const float2 none = two(0.0f);
+                store<IO, V>(gu_p + (t - t_e) * g.gu_t, none);
+                store<IO, V>(gd_p + (t - t_e) * g.gdelta_t, none);
+                if (g.grad_z) store<IO, V>(gz_p + (t - t_e) * g.gz_t, none);
             }
 
-        for (int t0 = (len - 1) / TT * TT; t0 >= 0 && len > 0; t0 -= TT) {
-            float u_r[E], dt_r[E], x_r[E], g_r[E], z_r[E];     // x: input of the softplus; g: grad_y
+        for (int t0 = top; t0 >= 0; t0 -= TT) {
+            const Raw& raw = sh.raw[t0 / TT & 1];
+            copy_wait<0>();
+            __syncthreads();
+            if (t0 >= TT) fill(t0 - TT);
+            float2 x_r[E], dt_r[E];                             // the softplus's argument and result
+            if (t_e < TT) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int tt = t_e + e * TS, t = t0 + tt;
-                const bool ok = ch_ok && tt < TT && t < len;
-                u_r[e] = ok ? to_f(u_p[t * a.u_t]) : 0.0f;
-                x_r[e] = ok ? to_f(d_p[t * a.delta_t]) + bias : 0.0f;
-                g_r[e] = ok ? to_f(gy_p[t * a.y_t]) : 0.0f;
-                if (GATE) z_r[e] = ok ? to_f(z_p[t * a.z_t]) : 0.0f;
-                dt_r[e] = a.softplus ? softplus_f(x_r[e]) : x_r[e];
-                if (!ok) dt_r[e] = 0.0f;
-                if (tt < TT) {
-                    s_dt[ch][tt] = dt_r[e];
-                    s_u[ch][tt] = u_r[e];
-                    s_g[ch][tt] = GATE ? g_r[e] * (z_r[e] * sigmoid_f(z_r[e])) : g_r[e];
+                for (int e = 0; e < E; ++e) {
+                    const int t = t_e + e * TS;
+                    const float2 u = unpack<IO, V>(&raw.u[t][ch]);
+                    float2 go = unpack<IO, V>(&raw.g[t][ch]);
+                    float2 dt = __fadd2_rn(unpack<IO, V>(&raw.d[t][ch]), bias);
+                    x_r[e] = dt;
+                    if (a.softplus) dt = softplus_f(dt);
+                    if (t0 + t >= len) dt = two(0.0f);          // a step behind the end leaves the state alone
+                    dt_r[e] = dt;
+                    if (a.z) {
+                        const float2 z = unpack<IO, V>(&raw.z[t][ch]);
+                        go = __fmul2_rn(go, __fmul2_rn(z, sigmoid_f(z)));
+                    }
+                    sh.d[ch][t] = make_float2(dt.x, dt.x * u.x);
+                    sh.g[ch][t] = go.x;
+                    if (V == 2) {
+                        sh.d[ch + V - 1][t] = make_float2(dt.y, dt.y * u.y);
+                        sh.g[ch + V - 1][t] = go.y;
+                    }
                 }
             }
 #pragma unroll
-            for (int f = 0; f < F; ++f) {
-                const int i = tid + f * NT, t = t0 + i / NS, n = i % NS;
-                const bool ok = i < TT * NS && n < a.states && t < len;
-                if (i < TT * NS) {
-                    s_B[n][i / NS] = ok ? to_f(B_p[t * a.B_t + n]) : 0.0f;
-                    s_C[n][i / NS] = ok ? to_f(C_p[t * a.C_t + n]) : 0.0f;
-                }
+            for (int i = tid; i < TT * NS; i += NT) {
+                sh.B[0][i] = to_f(raw.B[0][i]);
+                sh.C_[0][i] = to_f(raw.C_[0][i]);
             }
             __syncthreads();
 
-            // the chunk's decays and states
-            float da[C][S][TT], hh[C][S][TT + 1];
-            const float* kept = t0 > 0 ? a.kept + (long long)(t0 / TT - 1) * a.batch * a.channels * a.states
-                                       : a.h0;
+            // decays that stay near 1 for the whole tile take the polynomial (both of a pair, or none)
+            bool near1[C][J];
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c) {
+                float most = 0.0f;
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int n = s * SL + sl;
-                    const bool ok = c_base + warp * CL * C + c * CL + cl < p.group_channels && n < a.states;
-                    hh[c][s][0] = ok && kept ? kept[row0 + (long long)c * CL * a.states + n] : 0.0f;
-                }
-            float o[GATE ? C : 1][TT];
+                for (int t = 0; t < TT; t += SL)
+                    if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d[cl + c * CL][t + (SL <= TT ? sl : sl % TT)].x));
 #pragma unroll
-            for (int t4 = 0; t4 < TT; t4 += 4) {
-                float4 B4[S], C4[S];
+                for (int m = SL / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m * CL));
 #pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    B4[s] = *reinterpret_cast<const float4*>(&s_B[s * SL + sl][t4]);
-                    if (GATE) C4[s] = *reinterpret_cast<const float4*>(&s_C[s * SL + sl][t4]);
-                }
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int k = warp * CL * C + c * CL + cl;
-                    const float4 dt4 = *reinterpret_cast<const float4*>(&s_dt[k][t4]);
-                    const float4 u4 = *reinterpret_cast<const float4*>(&s_u[k][t4]);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const float dt = (&dt4.x)[t], du = dt * (&u4.x)[t];
-                        float acc = 0.0f;
-#pragma unroll
-                        for (int s = 0; s < S; ++s) {
-                            const float d = exp2_approx(dt * A2[c][s]);
-                            da[c][s][t4 + t] = d;
-                            hh[c][s][t4 + t + 1] = fmaf(d, hh[c][s][t4 + t], du * (&B4[s].x)[t]);
-                            if (GATE) acc = fmaf(hh[c][s][t4 + t + 1], (&C4[s].x)[t], acc);
-                        }
-                        if (GATE) o[c][t4 + t] = acc;
-                    }
-                }
-            }
-            if (GATE) {
-                using Sums = LaneSums<TT, SL, 1>;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    Sums::run(o[c], sl);
-                    if (Sums::stores(sl))
-#pragma unroll
-                        for (int i = 0; i < Sums::kHeld; ++i)
-                            s_o[warp * CL * C + c * CL + cl][Sums::first(sl) + i] = o[c][i];
-                }
+                for (int j = 0; j < J; ++j)
+                    near1[c][j] = most * fmaxf(fabsf(A2[c][j].x), fabsf(A2[c][j].y)) < kExp2Near;
             }
 
-            // and backwards through it, 8 steps at a time
-            constexpr int R = 8;
-#pragma unroll
+#pragma unroll 1
             for (int tr = TT - R; tr >= 0; tr -= R) {
-                float s1[C][R], s2[C][R];
+                if (t0 + tr >= len) continue;
+                // the 8 steps' decays and states
+                float2 da[R][C][J], hh[R + 1][C][J];
 #pragma unroll
-                for (int t4 = R - 4; t4 >= 0; t4 -= 4) {
-                    float4 B4[S], C4[S];
-                    float dB[S][4], dC[S][4];
+                for (int c = 0; c < C; ++c)
 #pragma unroll
-                    for (int s = 0; s < S; ++s) {
-                        B4[s] = *reinterpret_cast<const float4*>(&s_B[s * SL + sl][tr + t4]);
-                        C4[s] = *reinterpret_cast<const float4*>(&s_C[s * SL + sl][tr + t4]);
+                    for (int j = 0; j < J; ++j) hh[0][c][j] = start[c][j];
+                if (t0 + tr > 0) state_at(t0 + tr - R, start);
+                using OverStates = LaneSums<Q, SL, CL>;
+                using OverChannels = LaneSums<Q, CL, 1>;
+                auto keep = [&](float(&v)[Q], float* to) {
+                    OverStates::run(v, sl);
+                    if (OverStates::stores(sl)) {
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) dB[s][t] = dC[s][t] = 0.0f;
+                        for (int i = 0; i < OverStates::kHeld; ++i) to[OverStates::first(sl) + i] = v[i];
+                    }
+                };
+#pragma unroll
+                for (int tq = 0; tq < R; tq += Q) {
+                    float o[C][Q];
+#pragma unroll
+                    for (int i = 0; i < Q; ++i) {
+                        const int t = tq + i;
+                        float2 Bv[J], Cv[J];
+                        load_states<S>(Bv, &sh.B[tr + t][n0]);
+                        if (a.z) load_states<S>(Cv, &sh.C_[tr + t][n0]);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const float2 d = sh.d[cl + c * CL][tr + t];
+#pragma unroll
+                            for (int j = 0; j < J; ++j) {
+                                const float2 x = __fmul2_rn(two(d.x), A2[c][j]), q = exp2_near1(x);
+                                da[t][c][j] = make_float2(near1[c][j] ? q.x : exp2_approx(x.x),
+                                                          near1[c][j] ? q.y : exp2_approx(x.y));
+                                hh[t + 1][c][j] = __ffma2_rn(da[t][c][j], hh[t][c][j], __fmul2_rn(two(d.y), Bv[j]));
+                            }
+                            if (a.z) {
+                                float2 acc = __fmul2_rn(hh[t + 1][c][0], Cv[0]);
+#pragma unroll
+                                for (int j = 1; j < J; ++j) acc = __ffma2_rn(hh[t + 1][c][j], Cv[j], acc);
+                                o[c][i] = acc.x + acc.y;
+                            }
+                        }
+                    }
+                    if (a.z) {
+#pragma unroll
+                        for (int c = 0; c < C; ++c) keep(o[c], &sh.o[cl + c * CL][tr + tq]);
+                    }
+                }
+                // and backwards through them
+#pragma unroll
+                for (int tq = R - Q; tq >= 0; tq -= Q) {
+                    float lb[C][Q], qa[C][Q], dB[S][Q], dC[S][Q];
+#pragma unroll
+                    for (int i = Q - 1; i >= 0; --i) {
+                        const int t = tq + i;
+                        float2 Bv[J], Cv[J], dBt[J], dCt[J];
+                        load_states<S>(Bv, &sh.B[tr + t][n0]);
+                        load_states<S>(Cv, &sh.C_[tr + t][n0]);
+#pragma unroll
+                        for (int c = 0; c < C; ++c) {
+                            const float2 d = sh.d[cl + c * CL][tr + t];
+                            const float2 dt = two(d.x), du = two(d.y), go = two(sh.g[cl + c * CL][tr + t]);
+                            float2 r1, r2;
+#pragma unroll
+                            for (int j = 0; j < J; ++j) {
+                                const float2 l = __ffma2_rn(Cv[j], go, lam[c][j]);
+                                lam[c][j] = __fmul2_rn(l, da[t][c][j]);
+                                const float2 q = __fmul2_rn(lam[c][j], hh[t][c][j]);
+                                dBt[j] = c == 0 ? __fmul2_rn(l, du) : __ffma2_rn(l, du, dBt[j]);
+                                dCt[j] = c == 0 ? __fmul2_rn(go, hh[t + 1][c][j]) : __ffma2_rn(go, hh[t + 1][c][j], dCt[j]);
+                                r1 = j == 0 ? __fmul2_rn(l, Bv[j]) : __ffma2_rn(l, Bv[j], r1);
+                                r2 = j == 0 ? __fmul2_rn(q, A2[c][j]) : __ffma2_rn(q, A2[c][j], r2);
+                                dA[c][j] = __ffma2_rn(q, dt, dA[c][j]);
+                            }
+                            lb[c][i] = r1.x + r1.y;
+                            qa[c][i] = r2.x + r2.y;
+                        }
+#pragma unroll
+                        for (int j = 0; j < J; ++j) {
+                            dB[2 * j][i] = dBt[j].x;
+                            dB[2 * j + 1][i] = dBt[j].y;
+                            dC[2 * j][i] = dCt[j].x;
+                            dC[2 * j + 1][i] = dCt[j].y;
+                        }
                     }
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
-                        const int k = warp * CL * C + c * CL + cl;
-                        const float4 dt4 = *reinterpret_cast<const float4*>(&s_dt[k][tr + t4]);
-                        const float4 u4 = *reinterpret_cast<const float4*>(&s_u[k][tr + t4]);
-                        const float4 g4 = *reinterpret_cast<const float4*>(&s_g[k][tr + t4]);
-#pragma unroll
-                        for (int t = 3; t >= 0; --t) {
-                            const float dt = (&dt4.x)[t], du = dt * (&u4.x)[t], gt = (&g4.x)[t];
-                            float r1 = 0.0f, r2 = 0.0f;
-#pragma unroll
-                            for (int s = 0; s < S; ++s) {
-                                const float l = fmaf((&C4[s].x)[t], gt, lam[c][s]);
-                                lam[c][s] = l * da[c][s][tr + t4 + t];
-                                const float q = lam[c][s] * hh[c][s][tr + t4 + t];
-                                dB[s][t] = fmaf(l, du, dB[s][t]);
-                                dC[s][t] = fmaf(gt, hh[c][s][tr + t4 + t + 1], dC[s][t]);
-                                r1 = fmaf(l, (&B4[s].x)[t], r1);
-                                r2 = fmaf(q, A2[c][s], r2);
-                                dA[c][s] = fmaf(q, dt, dA[c][s]);
-                            }
-                            s1[c][t4 + t] = r1;
-                            s2[c][t4 + t] = r2;
-                        }
+                        keep(lb[c], &sh.lb[cl + c * CL][tr + tq]);
+                        keep(qa[c], &sh.qa[cl + c * CL][tr + tq]);
                     }
-                    using Sums = LaneSums<4, CL, SL>;
 #pragma unroll
                     for (int s = 0; s < S; ++s) {
-                        Sums::run(dB[s], cl);
-                        Sums::run(dC[s], cl);
-                        if (Sums::stores(cl)) {
-#pragma unroll
-                            for (int i = 0; i < Sums::kHeld; ++i) {
-                                const int t = tr + t4 + Sums::first(cl) + i, n = s * SL + sl;
-                                s_red[((warp * 2 + 0) * TT + t) * NS + n] = dB[s][i];
-                                s_red[((warp * 2 + 1) * TT + t) * NS + n] = dC[s][i];
-                            }
-                        }
+                        OverChannels::run(dB[s], lc);
+                        OverChannels::run(dC[s], lc);
                     }
-                }
-                using Sums = LaneSums<R, SL, 1>;
-                __syncwarp();
+                    if (OverChannels::stores(lc)) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    Sums::run(s1[c], sl);
-                    Sums::run(s2[c], sl);
-                    // the sums go where this warp's d and u of these steps were
-                    if (Sums::stores(sl)) {
-                        const int k = warp * CL * C + c * CL + cl;
-#pragma unroll
-                        for (int i = 0; i < Sums::kHeld; ++i) {
-                            s_dt[k][tr + Sums::first(sl) + i] = s1[c][i];
-                            s_u[k][tr + Sums::first(sl) + i] = s2[c][i];
+                        for (int i = 0; i < OverChannels::kHeld; ++i) {
+                            const int t = tr + tq + OverChannels::first(lc) + i;
+                            store_states<S>(&sh.red[warp][0][t][n0], dB, i);
+                            store_states<S>(&sh.red[warp][1][t][n0], dC, i);
                         }
                     }
                 }
@@ -272,73 +354,76 @@ __global__ void __launch_bounds__(NT) scan_bwd(const ScanParams p) {
             if (ch_ok) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    const int tt = t_e + e * TS, t = t0 + tt;
-                    if (tt < TT && t < p.T) {
-                        const float lb = s_dt[ch][tt], qa = s_u[ch][tt] * 0.69314718055994530942f;
-                        float gt = g_r[e], gz = 0.0f;
-                        if (GATE) {
-                            const float sg = sigmoid_f(z_r[e]), si = z_r[e] * sg;
-                            gz = gt * fmaf(skip, u_r[e], s_o[ch][tt]) * fmaf(si, 1.0f - sg, sg);
-                            gt *= si;
+                    const int t = t_e + e * TS;
+                    if (t0 + t < p.T) {
+                        const float2 u = unpack<IO, V>(&raw.u[t][ch]);
+                        float2 go = unpack<IO, V>(&raw.g[t][ch]), gz = two(0.0f);
+                        const float2 lb = make_float2(sh.lb[ch][t], sh.lb[ch + V - 1][t]);
+                        const float2 qa = make_float2(sh.qa[ch][t], sh.qa[ch + V - 1][t]);
+                        if (a.z) {
+                            const float2 z = unpack<IO, V>(&raw.z[t][ch]), sg = sigmoid_f(z), si = __fmul2_rn(z, sg);
+                            const float2 o = __ffma2_rn(skip, u, make_float2(sh.o[ch][t], sh.o[ch + V - 1][t]));
+                            // silu' = sg + si (1 - sg)
+                            const float2 ds = __ffma2_rn(si, __ffma2_rn(sg, two(-1.0f), two(1.0f)), sg);
+                            gz = __fmul2_rn(__fmul2_rn(go, o), ds);
+                            go = __fmul2_rn(go, si);
                         }
-                        float gd = fmaf(u_r[e], lb, qa);
-                        if (a.softplus) gd *= sigmoid_f(x_r[e]);
-                        float gu = fmaf(dt_r[e], lb, skip * gt);
-                        if (t >= len) gd = gu = gz = 0.0f;
-                        gu_p[t * g.gu_t] = from_f<IO>(gu);
-                        gd_p[t * g.gdelta_t] = from_f<IO>(gd);
-                        if (GATE && gz_p) gz_p[t * g.gz_t] = from_f<IO>(gz);
-                        sum_bias += gd;
-                        sum_D = fmaf(gt, u_r[e], sum_D);
+                        // q A came with A log2 e
+                        float2 gd = __ffma2_rn(u, lb, __fmul2_rn(qa, two(0.69314718055994530942f)));
+                        if (a.softplus) gd = __fmul2_rn(gd, sigmoid_f(x_r[e]));
+                        float2 gu = __ffma2_rn(dt_r[e], lb, __fmul2_rn(skip, go));
+                        if (t0 + t >= len) gd = gu = gz = go = two(0.0f);
+                        store<IO, V>(gu_p + (t0 + e * TS) * g.gu_t, gu);
+                        store<IO, V>(gd_p + (t0 + e * TS) * g.gdelta_t, gd);
+                        if (g.grad_z) store<IO, V>(gz_p + (t0 + e * TS) * g.gz_t, gz);
+                        sum_bias = __fadd2_rn(sum_bias, gd);
+                        if (t0 + t < len) sum_D = __ffma2_rn(go, u, sum_D);
                     }
                 }
             }
             // this block's part of grad B and grad C
-            for (int i = tid; i < 2 * TT * NS; i += NT) {
-                const int n = i % NS, t = t0 + i / NS % TT, which = i / (NS * TT);
-                if (n < a.states && t < len) {
-                    float v = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < NW; ++w) v += s_red[w * 2 * TT * NS + i];
-                    p.part_bc[((((long long)which * p.tiles + tile) * p.T + t) * a.batch + b) * a.groups * a.states
-                              + grp * a.states + n] = v;
+            for (int i = tid; i < 2 * TT * NS / S; i += NT) {
+                const int n = i % (NS / S) * S, t = i / (NS / S) % TT, which = i / (NS / S * TT);
+                if (t0 + t < len) {
+                    float2 v[J];
+                    load_states<S>(v, &sh.red[0][which][t][n]);
+#pragma unroll
+                    for (int w = 1; w < NW; ++w) {
+                        float2 x[J];
+                        load_states<S>(x, &sh.red[w][which][t][n]);
+#pragma unroll
+                        for (int j = 0; j < J; ++j) v[j] = __fadd2_rn(v[j], x[j]);
+                    }
+                    float* q = p.part_bc + ((((long long)which * p.tiles + tile) * p.T + t0 + t) * a.batch + b) * a.groups * a.states
+                               + grp * a.states + n;
+#pragma unroll
+                    for (int s = 0; s < S; ++s)
+                        if (n + s < a.states) q[s] = s % 2 ? v[s / 2].y : v[s / 2].x;
                 }
             }
-            __syncthreads();
         }
-        if (g.grad_h0) {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int s = 0; s < S; ++s) {
-                    const int n = s * SL + sl;
-                    if (c_base + warp * CL * C + c * CL + cl < p.group_channels && n < a.states)
-                        g.grad_h0[row0 + (long long)c * CL * a.states + n] = lam[c][s];
-                }
-        }
+        if (g.grad_h0) put(g.grad_h0 + row, lam);
+        __syncthreads();                                        // before the next sequence's copies
     }
 
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int k = c_base + warp * CL * C + c * CL + cl, n = s * SL + sl;
-            if (k < p.group_channels && n < a.states)
-                p.part_a[((long long)part * a.channels + g_base + k) * a.states + n] = dA[c][s];
-        }
+    put(p.part_a + ((long long)part * a.channels + g_base + c_base + cl) * a.states + n0, dA);
     // the threads of a channel, in order
-    __syncthreads();
-    smem[tid] = sum_D;
-    smem[NT + tid] = sum_bias;
-    __syncthreads();
-    if (tid < BC && c_base + tid < p.group_channels) {
-        float d = 0.0f, e = 0.0f;
-        for (int i = tid; i < NT; i += BC) {
-            d += smem[i];
-            e += smem[NT + i];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        __syncthreads();
+        sh.sums[0][tid] = v ? sum_D.y : sum_D.x;
+        sh.sums[1][tid] = v ? sum_bias.y : sum_bias.x;
+        __syncthreads();
+        if (tid < ROW && ch + v < cols) {
+            float d = 0.0f, e = 0.0f;
+            for (int i = tid; i < NT; i += ROW) {
+                d += sh.sums[0][i];
+                e += sh.sums[1][i];
+            }
+            p.part_d[(long long)part * a.channels + chan + v] = d;
+            p.part_d[((long long)p.batch_parts + part) * a.channels + chan + v] = e;
         }
-        p.part_d[(long long)part * a.channels + chan] = d;
-        p.part_d[((long long)p.batch_parts + part) * a.channels + chan] = e;
     }
 }
 
@@ -378,43 +463,39 @@ __global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a)
     }
 }
 
-// Channels of a block for a state count (the shapes that pick() launches)
-int block_channels(int states) {
-    if (states <= 4) return Shape<4, 1, 1>::BC;
-    if (states <= 8) return Shape<2, 2, 4>::BC;
-    if (states <= 16) return Shape<2, 2, 8>::BC;
-    if (states <= 32) return Shape<2, 2, 16>::BC;
-    if (states <= 64) return Shape<2, 2, 32>::BC;
-    return Shape<4, 1, 32>::BC;
-}
-
-template <typename IO, int S, int C, int SL, bool GATE>
-cudaError_t launch_gate(const ScanParams& p, cudaStream_t st) {
+template <typename IO, int S, int SL, int C, bool WIDE>
+cudaError_t launch_form(const ScanParams& p, cudaStream_t st) {
     const long long blocks = (long long)p.tiles * p.a.groups * p.batch_parts;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    constexpr size_t smem = Shape<S, C, SL>::smem(GATE);
-    cudaError_t e = cudaFuncSetAttribute(scan_bwd<IO, S, C, SL, GATE>,
+    constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
+    cudaError_t e = cudaFuncSetAttribute(scan_bwd<IO, S, SL, C, WIDE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    scan_bwd<IO, S, C, SL, GATE><<<(unsigned)blocks, NT, smem, st>>>(p);
+    scan_bwd<IO, S, SL, C, WIDE><<<(unsigned)blocks, NT, smem, st>>>(p);
     return cudaGetLastError();
 }
 
-template <typename IO, int S, int C, int SL>
-cudaError_t launch(const ScanParams& p, cudaStream_t st) {
-    return p.a.z ? launch_gate<IO, S, C, SL, true>(p, st) : launch_gate<IO, S, C, SL, false>(p, st);
+template <typename IO, int S, int SL, int C>
+cudaError_t launch(ScanParams p, cudaStream_t st) {
+    const dfsnn_state_scan_grads& g = p.g;
+    p.words = rows_aligned(p, sizeof(IO), 4);
+    const bool wide = p.group_channels % 2 == 0 && rows_aligned(p, sizeof(IO), 16)
+                      && pairs_aligned(g.grad_u, g.gu_t, g.gu_b, sizeof(IO))
+                      && pairs_aligned(g.grad_delta, g.gdelta_t, g.gdelta_b, sizeof(IO))
+                      && pairs_aligned(g.grad_z, g.gz_t, g.gz_b, sizeof(IO));
+    return wide ? launch_form<IO, S, SL, C, true>(p, st) : launch_form<IO, S, SL, C, false>(p, st);
 }
 
 template <typename IO>
 cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     const int n = p.a.states;
     cudaError_t e;
-    if (n <= 4) e = launch<IO, 4, 1, 1>(p, st);
-    else if (n <= 8) e = launch<IO, 2, 2, 4>(p, st);
-    else if (n <= 16) e = launch<IO, 2, 2, 8>(p, st);
-    else if (n <= 32) e = launch<IO, 2, 2, 16>(p, st);
-    else if (n <= 64) e = launch<IO, 2, 2, 32>(p, st);
-    else e = launch<IO, 4, 1, 32>(p, st);
+    if (n <= 4) e = launch<IO, 2, 2, 1>(p, st);
+    else if (n <= 8) e = launch<IO, 2, 4, 2>(p, st);
+    else if (n <= 16) e = launch<IO, 4, 4, 2>(p, st);
+    else if (n <= 32) e = launch<IO, 4, 8, 2>(p, st);
+    else if (n <= 64) e = launch<IO, 4, 16, 2>(p, st);
+    else e = launch<IO, 4, 32, 2>(p, st);
     if (e != cudaSuccess) return e;
     const long long n_bc = (long long)p.T * p.a.batch * p.a.groups * p.a.states;
     const long long n_a = p.a.channels * p.a.states;
@@ -424,6 +505,16 @@ cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     return cudaGetLastError();
 }
 
+// Channels of a block for a state count, as pick() has them
+int block_channels(int states) {
+    if (states <= 4) return Tile<float, 2, 2, 1>::BC;
+    if (states <= 8) return Tile<float, 2, 4, 2>::BC;
+    if (states <= 16) return Tile<float, 4, 4, 2>::BC;
+    if (states <= 32) return Tile<float, 4, 8, 2>::BC;
+    if (states <= 64) return Tile<float, 4, 16, 2>::BC;
+    return Tile<float, 4, 32, 2>::BC;
+}
+
 }  // namespace
 
 int state_scan_bwd_tiles(int states, long long group_channels) {
@@ -431,11 +522,11 @@ int state_scan_bwd_tiles(int states, long long group_channels) {
     return (int)((group_channels + bc - 1) / bc);
 }
 
-// Blocks that share the batch: enough for 16 blocks an SM; beyond that each block takes several
+// Blocks that share the batch: enough for 8 blocks an SM; beyond that each block takes several
 // sequences and adds its grad A on the way, which keeps the partial sums small.
 int state_scan_bwd_batch_parts(int states, long long batch, long long group_channels, int groups) {
     const long long per = (long long)state_scan_bwd_tiles(states, group_channels) * groups;
-    const long long want = (148 * 16 + per - 1) / per;
+    const long long want = (148 * 8 + per - 1) / per;
     return (int)std::max<long long>(1, std::min(batch, want));
 }
 

@@ -26,7 +26,7 @@
 namespace dfsnn {
 namespace {
 
-constexpr int TT = kScanChunk, NT = 128;
+constexpr int TT = kScanTile, NT = 128;
 
 // S states on each of a channel's SL lanes, C channels a lane
 template <typename IO, int S, int SL, int C>
@@ -129,15 +129,15 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
     auto fill = [&](int t0) {
         const int stage = (t0 - first) / TT & 1, rows = len - t0;
         if constexpr (WIDE) {
-            pieces.template issue<Tl::kEights>(stage * (unsigned)sizeof(Raw), rows);
+            pieces.template issue<Tl::kEights, 1>(stage * (unsigned)sizeof(Raw), rows);
         } else {
             Raw& r = sh.raw[stage];
-            fill_tile<IO, TT, BC, NT>(r.u[0], u_p, a.u_t, rows, cols, p.words);
-            fill_tile<IO, TT, BC, NT>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
-            fill_tile<IO, TT, NS, NT>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+            fill_tile<IO, TT, BC, NT, false>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, false>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT, false>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
             if (!ENDS) {
-                if (a.z) fill_tile<IO, TT, BC, NT>(r.z[0], z_p, a.z_t, rows, cols, p.words);
-                fill_tile<IO, TT, NS, NT>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+                if (a.z) fill_tile<IO, TT, BC, NT, false>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+                fill_tile<IO, TT, NS, NT, false>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
             }
             u_p += TT * a.u_t;
             d_p += TT * a.delta_t;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
 
     for (int t0 = first; t0 < len; t0 += TT) {
         const Raw& raw = sh.raw[(t0 - first) / TT & 1];
-        copy_wait_all();
+        copy_wait<0>();
         __syncthreads();
         if (t0 + TT < len) fill(t0 + TT);
         if (t_e < TT) {
@@ -234,8 +234,6 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
             if (!ENDS) sh.C_[0][i] = to_f(raw.C_[0][i]);
         }
         __syncthreads();
-        if (!ENDS && a.kept && t0 > 0)
-            put(a.kept + (long long)(t0 / TT - 1) * a.batch * a.channels * a.states + row);
         // decays that stay near 1 for the whole tile take the polynomial
         bool near1[C][S];
 #pragma unroll
@@ -255,6 +253,9 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
         constexpr int R = 8;                    // steps whose sums over the lanes are formed together
 #pragma unroll
         for (int tr = 0; tr < TT; tr += R) {
+            static_assert(R == kScanChunk, "states are kept in front of every R steps");
+            if (!ENDS && a.kept && t0 + tr > 0 && t0 + tr < len)
+                put(a.kept + (long long)((t0 + tr) / R - 1) * a.batch * a.channels * a.states + row);
             float y[C][R];
             constexpr int G = 4;                // steps whose decays are formed before their states
 #pragma unroll
@@ -374,8 +375,7 @@ cudaError_t launch(ScanParams p, cudaStream_t st) {
     if (blocks > 0x7fffffffLL / p.splits) return cudaErrorInvalidValue;
     const dfsnn_state_scan_args& a = p.a;
     p.words = rows_aligned(p, sizeof(IO), 4);
-    const bool pairs = p.group_channels % 2 == 0 && reinterpret_cast<uintptr_t>(a.y) % (2 * sizeof(IO)) == 0 && a.y_t % 2 == 0 && a.y_b % 2 == 0;
-    return pairs && rows_aligned(p, sizeof(IO), 16) ? launch_form<IO, S, SL, C, true>(p, (unsigned)blocks, st)
+    return p.group_channels % 2 == 0 && pairs_aligned(a.y, a.y_t, a.y_b, sizeof(IO)) && rows_aligned(p, sizeof(IO), 16) ? launch_form<IO, S, SL, C, true>(p, (unsigned)blocks, st)
                                                     : launch_form<IO, S, SL, C, false>(p, (unsigned)blocks, st);
 }
 

@@ -15,21 +15,27 @@ __device__ __forceinline__ void copy_async(void* dst, const void* src, int bytes
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+// until all but the newest LEFT groups of this thread have landed
+template <int LEFT>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// A tile of ROWS steps x COLS neighbouring elements, by the NT threads of a block, element by
-// element: steps from `rows` and elements from `cols` on become zero and are not read.  `words`:
-// every row starts on a 4-byte boundary and is copied asynchronously, 4 bytes at a time.
-template <typename IO, int ROWS, int COLS, int NT>
+// A tile of ROWS steps x COLS neighbouring elements, by the NT threads of a block: steps from
+// `rows` and elements from `cols` on become zero and are not read.  WIDE: rows start on 16-byte
+// boundaries and are copied 16 bytes at a time (8 where a row of the tile has no more).  Otherwise
+// `words` says that every row starts on a 4-byte boundary; rows that do not (odd offsets of 16-bit
+// types) are loaded and stored.
+template <typename IO, int ROWS, int COLS, int NT, bool WIDE>
 __device__ __forceinline__ void fill_tile(IO* dst, const IO* src, long long stride, int rows, int cols, bool words) {
-    constexpr int E = (int)sizeof(IO), PER = 4 / E, CPR = COLS / PER;
-    if (words) {
+    constexpr int E = (int)sizeof(IO);
+    constexpr int BYTES = !WIDE ? 4 : COLS * E >= 16 ? 16 : COLS * E;
+    constexpr int PER = BYTES / E, CPR = COLS / PER;
+    if (WIDE || words) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < ROWS * CPR; i += NT) {
             const int t = i / CPR, c = i % CPR * PER;
             int n = t < rows ? (cols - c) * E : 0;
-            n = n < 0 ? 0 : n > 4 ? 4 : n;
-            copy_async<4>(dst + t * COLS + c, n ? src + t * stride + c : src, n);
+            n = n < 0 ? 0 : n > BYTES ? BYTES : n;
+            copy_async<BYTES>(dst + t * COLS + c, n ? src + t * stride + c : src, n);
         }
     } else {
 #pragma unroll 4
@@ -79,8 +85,9 @@ struct TilePieces {
         }
         next += ROWS * CPR;
     }
-    // copies of the current tile to the stage `offset` bytes on, and on to the next tile
-    template <bool EIGHTS>
+    // copies of the current tile to the stage `offset` bytes on, and on to the next tile (DIRECTION
+    // 1) or the one in front (-1)
+    template <bool EIGHTS, int DIRECTION>
     __device__ __forceinline__ void issue(unsigned offset, int rows) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -90,7 +97,7 @@ struct TilePieces {
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst[k] + offset), "l"(src[k]), "r"(bytes) : "memory");
                 else
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst[k] + offset), "l"(src[k]), "r"(bytes) : "memory");
-                src[k] += step[k];
+                src[k] += DIRECTION * step[k];
             }
         }
     }

@@ -42,7 +42,7 @@ STATE_SCAN_STEP_ARGS = struct.Struct("<12Q13q6i")
 SHORT_CONV_ARGS = struct.Struct("<7Q7q4i")
 SHORT_CONV_GRADS = struct.Struct("<6Q2q")
 SHORT_CONV_STEP_ARGS = struct.Struct("<7Q7q4i")
-SCAN_MAX_STATES, SCAN_CHUNK, CONV_MAX_TAPS = 128, 16, 8
+SCAN_MAX_STATES, SCAN_CHUNK, CONV_MAX_TAPS = 128, 8, 8
 
 # name -> (restype, argtypes)
 SIGNATURES = {

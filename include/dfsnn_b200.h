@@ -376,7 +376,7 @@ int dfsnn_check_surrogate_quotient(const float* a, int n_numerators, int exp_lo,
  * ------------------------------------------------------------------------------- */
 
 #define DFSNN_SCAN_MAX_STATES 128   /* states per channel */
-#define DFSNN_SCAN_CHUNK 16         /* steps between the states that the forward keeps */
+#define DFSNN_SCAN_CHUNK 8          /* steps between the states that the forward keeps */
 #define DFSNN_CONV_MAX_TAPS 8
 
 /* Selective scan, per sequence b, channel c (of group c / (channels / groups)) and state n:
