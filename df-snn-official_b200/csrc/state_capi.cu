@@ -55,18 +55,20 @@ dfsnn::ScanParams scan_params(const dfsnn_state_scan_args& a) {
 }
 
 struct ScanWorkspace {
-    int tiles, parts;
-    size_t bc, a, d;        // floats
-    size_t bytes() const { return (bc + a + d) * sizeof(float); }
+    size_t bc, a, d, ends, end_steps;       // floats
+    size_t bytes() const { return (bc + a + d + ends + end_steps) * sizeof(float); }
 };
 
-ScanWorkspace scan_workspace(long long T, long long batch, long long channels, int states, int groups) {
+ScanWorkspace backward_plan(dfsnn::ScanParams& p) {
+    p.tiles = dfsnn::state_scan_bwd_tiles(p.a.states, p.group_channels);
+    dfsnn::state_scan_bwd_plan(p);
+    const size_t rows = (size_t)p.a.batch * p.a.channels, parts = (size_t)p.batch_parts * p.splits;
     ScanWorkspace w;
-    w.tiles = dfsnn::state_scan_bwd_tiles(states, channels / groups);
-    w.parts = dfsnn::state_scan_bwd_batch_parts(states, batch, channels / groups, groups);
-    w.bc = (size_t)2 * w.tiles * T * batch * groups * states;
-    w.a = (size_t)w.parts * channels * states;
-    w.d = (size_t)2 * w.parts * channels;
+    w.bc = (size_t)2 * p.tiles * p.a.T * p.a.batch * p.a.groups * p.a.states;
+    w.a = parts * p.a.channels * p.a.states;
+    w.d = 2 * parts * p.a.channels;
+    w.ends = p.splits > 1 ? p.splits * rows * p.a.states : 0;
+    w.end_steps = p.splits > 1 ? p.splits * rows : 0;
     return w;
 }
 
@@ -109,7 +111,14 @@ int dfsnn_state_scan_forward(const dfsnn_state_scan_args* a, void* workspace, si
 size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,
                                                 int states, int groups) {
     if (check_scan_sizes(T, batch, channels, states, groups) || batch == 0 || channels == 0) return 0;
-    return scan_workspace(T, batch, channels, states, groups).bytes();
+    dfsnn_state_scan_args a{};
+    a.T = T;
+    a.batch = batch;
+    a.channels = channels;
+    a.states = states;
+    a.groups = groups;
+    dfsnn::ScanParams p = scan_params(a);
+    return backward_plan(p).bytes();
 }
 
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g,
@@ -121,15 +130,15 @@ int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_
         || !g->grad_B || !g->grad_C || !g->grad_A)
         return DFSNN_ERR_NULL;
     if (!a->kept && a->T > DFSNN_SCAN_CHUNK) return DFSNN_ERR_NULL;
-    const ScanWorkspace w = scan_workspace(a->T, a->batch, a->channels, a->states, a->groups);
-    if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return DFSNN_ERR_WORKSPACE;
     dfsnn::ScanParams p = scan_params(*a);
     p.g = *g;
-    p.tiles = w.tiles;
-    p.batch_parts = w.parts;
+    const ScanWorkspace w = backward_plan(p);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return DFSNN_ERR_WORKSPACE;
     p.part_bc = static_cast<float*>(workspace);
     p.part_a = p.part_bc + w.bc;
     p.part_d = p.part_a + w.a;
+    p.ends = p.part_d + w.d;
+    p.end_steps = p.ends + w.ends;
     return status(dfsnn::state_scan_backward_launch(p, (cudaStream_t)stream));
 }
 

@@ -15,13 +15,13 @@ struct ScanParams {
     bool words;                                // rows_aligned(4), for rows that are not on 16 bytes
     // a sequence in parts (splits > 1): `split_steps` steps each, a multiple of the chunk
     int splits, split_steps;
-    float* ends;                               // [splits - 1][batch][channels][states]
-    float* end_steps;                          // [splits - 1][batch][channels] sums of d
+    float* ends;                               // [splits][batch][channels][states] (forward: all but
+    float* end_steps;                          // the last, backward: the first unused) and sums of d
     // backward
     int batch_parts;                           // blocks that share the batch (part q: b = q, q + parts, ...)
     float* part_bc;                            // [2][tiles][T][batch][groups][states]
-    float* part_a;                             // [batch_parts][channels][states]
-    float* part_d;                             // [2][batch_parts][channels] (D, delta_bias)
+    float* part_a;                             // [batch_parts * splits][channels][states]
+    float* part_d;                             // [2][batch_parts * splits][channels] (D, delta_bias)
 };
 
 // Whether every row (a step's channels of a group, a step's states) of the inputs starts on a
@@ -45,7 +45,7 @@ inline bool pairs_aligned(const void* q, long long t, long long b, size_t elem) 
 int state_scan_splits(long long T, long long batch, long long group_channels, int groups, int states);
 cudaError_t state_scan_forward_launch(const ScanParams& p, cudaStream_t st);
 int state_scan_bwd_tiles(int states, long long group_channels);
-int state_scan_bwd_batch_parts(int states, long long batch, long long group_channels, int groups);
+void state_scan_bwd_plan(ScanParams& p);       // sets splits, split_steps and batch_parts
 cudaError_t state_scan_backward_launch(const ScanParams& p, cudaStream_t st);
 
 }  // namespace dfsnn

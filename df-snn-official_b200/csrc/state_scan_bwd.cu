@@ -80,7 +80,7 @@ __device__ __forceinline__ void store(IO* q, float2 f) {
 }
 
 template <typename IO, int S, int SL, int C, bool WIDE>
-__global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
+__global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
     using Tl = Tile<IO, S, SL, C>;
     constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS, J = S / 2;
     constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
@@ -97,7 +97,11 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
     const int tile = (int)(bid % p.tiles);
     bid /= p.tiles;
     const int grp = (int)(bid % a.groups);
-    const int part = (int)(bid / a.groups);
+    bid /= a.groups;
+    const int split = (int)(bid % p.splits), batch_part = (int)(bid / p.splits);
+    const int first = split * p.split_steps;                    // this part's steps: first .. stop - 1
+    const int stop = p.T - first < p.split_steps ? p.T : first + p.split_steps;
+    const int part = batch_part * p.splits + split, parts = p.batch_parts * p.splits;
     const int c_base = tile * BC, cols = p.group_channels - c_base;
     const long long g_base = (long long)grp * p.group_channels;
 
@@ -112,6 +116,9 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
     // recurrence role: states n0 .. n0 + S - 1 of channels cl + c * CL of the block
     const int sl = lane / CL, lc = lane % CL, cl = warp * CW + lc, n0 = sl * S;
     const long long crow = (long long)CL * a.states;
+    // a lane's states are one access everywhere
+    const bool whole = S == 4 && a.states % 4 == 0
+                       && ((reinterpret_cast<uintptr_t>(a.kept) | reinterpret_cast<uintptr_t>(a.h0)) & 15) == 0;
     auto get = [&](const float* q, float2(&v)[C][J]) {
 #pragma unroll
         for (int c = 0; c < C; ++c)
@@ -135,9 +142,10 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
 #pragma unroll
         for (int j = 0; j < J; ++j) A2[c][j] = __fmul2_rn(A2[c][j], two(kLog2e));
 
-    for (long long b = part; b < a.batch; b += p.batch_parts) {
-        const int len = seq_length(a.lengths, a.lengths64, b, p.T);
-        const int top = len > 0 ? (len - 1) / TT * TT : -1;     // first step of the last tile
+    for (long long b = batch_part; b < a.batch; b += p.batch_parts) {
+        const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T);
+        const int len = whole_len < stop ? whole_len : stop;
+        const int top = len > first ? (len - 1) / TT * TT : -1; // first step of the last tile
         IO* gu_p = static_cast<IO*>(g.grad_u) + b * g.gu_b + chan + t_e * g.gu_t;
         IO* gd_p = static_cast<IO*>(g.grad_delta) + b * g.gdelta_b + chan + t_e * g.gdelta_t;
         IO* gz_p = static_cast<IO*>(g.grad_z) + b * g.gz_b + chan + t_e * g.gz_t;
@@ -172,28 +180,50 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
 
         // the state in front of the 8 steps from t on
         auto state_at = [&](int t, float2(&v)[C][J]) {
-            get(t > 0 ? a.kept + (long long)(t / R - 1) * a.batch * a.channels * a.states + row
-                      : (a.h0 ? a.h0 + row : nullptr), v);
+            const float* q = t > 0 ? a.kept + (long long)(t / R - 1) * a.batch * a.channels * a.states + row
+                                   : (a.h0 ? a.h0 + row : nullptr);
+            if (whole && q) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+                    if (cl + c * CL < cols && n0 < a.states) load_states<S>(v[c], q + c * crow);
+            } else {
+                get(q, v);
+            }
         };
         float2 start[C][J] = {};                                // loaded one chunk ahead
         if (top >= 0) state_at((len - 1) / R * R, start);
         float2 lam[C][J] = {};                                  // a_(t+1) l_(t+1)
-        get(g.grad_h_last ? g.grad_h_last + row : nullptr, lam);
+        if (len > first || split == 0) {
+            get(g.grad_h_last ? g.grad_h_last + row : nullptr, lam);
+            const long long rows = a.batch * a.channels;
+            for (int k = (whole_len - 1) / p.split_steps; k > split; --k) {
+                float2 end[C][J] = {};
+                get(p.ends + k * rows * a.states + row, end);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const float d = cl + c * CL < cols ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < J; ++j)
+                        lam[c][j] = make_float2(fmaf(exp2_approx(d * A2[c][j].x), lam[c][j].x, end[c][j].x),
+                                                fmaf(exp2_approx(d * A2[c][j].y), lam[c][j].y, end[c][j].y));
+                }
+            }
+        }
 
         // rows behind the end
         if (ch_ok)
-            for (long long t = (long long)top + (top < 0 ? 1 : TT) + t_e; t < p.T; t += TS) {
+            for (long long t = (top < 0 ? (long long)first : (long long)top + TT) + t_e; t < stop; t += TS) {
                 const float2 none = two(0.0f);
                 store<IO, V>(gu_p + (t - t_e) * g.gu_t, none);
                 store<IO, V>(gd_p + (t - t_e) * g.gdelta_t, none);
                 if (g.grad_z) store<IO, V>(gz_p + (t - t_e) * g.gz_t, none);
             }
 
-        for (int t0 = top; t0 >= 0; t0 -= TT) {
+        for (int t0 = top; t0 >= first; t0 -= TT) {
             const Raw& raw = sh.raw[t0 / TT & 1];
             copy_wait<0>();
             __syncthreads();
-            if (t0 >= TT) fill(t0 - TT);
+            if (t0 > first) fill(t0 - TT);
             float2 x_r[E], dt_r[E];                             // the softplus's argument and result
             if (t_e < TT) {
 #pragma unroll
@@ -249,7 +279,7 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                 for (int c = 0; c < C; ++c)
 #pragma unroll
                     for (int j = 0; j < J; ++j) hh[0][c][j] = start[c][j];
-                if (t0 + tr > 0) state_at(t0 + tr - R, start);
+                if (t0 + tr > first) state_at(t0 + tr - R, start);
                 using OverStates = LaneSums<Q, SL, CL>;
                 using OverChannels = LaneSums<Q, CL, 1>;
                 auto keep = [&](float(&v)[Q], float* to) {
@@ -259,24 +289,34 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                         for (int i = 0; i < OverStates::kHeld; ++i) to[OverStates::first(sl) + i] = v[i];
                     }
                 };
+                auto over_channels = [&](float(&v)[S][Q], float(*to)[NS], int tq) {
+#pragma unroll
+                    for (int s = 0; s < S; ++s) OverChannels::run(v[s], lc);
+                    if (OverChannels::stores(lc)) {
+#pragma unroll
+                        for (int i = 0; i < OverChannels::kHeld; ++i)
+                            store_states<S>(&to[tr + tq + OverChannels::first(lc) + i][n0], v, i);
+                    }
+                };
 #pragma unroll
                 for (int tq = 0; tq < R; tq += Q) {
-                    float o[C][Q];
+                    float o[C][Q], dC[S][Q];
 #pragma unroll
                     for (int i = 0; i < Q; ++i) {
                         const int t = tq + i;
-                        float2 Bv[J], Cv[J];
+                        float2 Bv[J], Cv[J], dCt[J];
                         load_states<S>(Bv, &sh.B[tr + t][n0]);
                         if (a.z) load_states<S>(Cv, &sh.C_[tr + t][n0]);
 #pragma unroll
                         for (int c = 0; c < C; ++c) {
-                            const float2 d = sh.d[cl + c * CL][tr + t];
+                            const float2 d = sh.d[cl + c * CL][tr + t], go = two(sh.g[cl + c * CL][tr + t]);
 #pragma unroll
                             for (int j = 0; j < J; ++j) {
                                 const float2 x = __fmul2_rn(two(d.x), A2[c][j]), q = exp2_near1(x);
                                 da[t][c][j] = make_float2(near1[c][j] ? q.x : exp2_approx(x.x),
                                                           near1[c][j] ? q.y : exp2_approx(x.y));
                                 hh[t + 1][c][j] = __ffma2_rn(da[t][c][j], hh[t][c][j], __fmul2_rn(two(d.y), Bv[j]));
+                                dCt[j] = c == 0 ? __fmul2_rn(go, hh[t + 1][c][j]) : __ffma2_rn(go, hh[t + 1][c][j], dCt[j]);
                             }
                             if (a.z) {
                                 float2 acc = __fmul2_rn(hh[t + 1][c][0], Cv[0]);
@@ -285,7 +325,13 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                                 o[c][i] = acc.x + acc.y;
                             }
                         }
+#pragma unroll
+                        for (int j = 0; j < J; ++j) {
+                            dC[2 * j][i] = dCt[j].x;
+                            dC[2 * j + 1][i] = dCt[j].y;
+                        }
                     }
+                    over_channels(dC, sh.red[warp][1], tq);
                     if (a.z) {
 #pragma unroll
                         for (int c = 0; c < C; ++c) keep(o[c], &sh.o[cl + c * CL][tr + tq]);
@@ -294,11 +340,11 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                 // and backwards through them
 #pragma unroll
                 for (int tq = R - Q; tq >= 0; tq -= Q) {
-                    float lb[C][Q], qa[C][Q], dB[S][Q], dC[S][Q];
+                    float lb[C][Q], qa[C][Q], dB[S][Q];
 #pragma unroll
                     for (int i = Q - 1; i >= 0; --i) {
                         const int t = tq + i;
-                        float2 Bv[J], Cv[J], dBt[J], dCt[J];
+                        float2 Bv[J], Cv[J], dBt[J];
                         load_states<S>(Bv, &sh.B[tr + t][n0]);
                         load_states<S>(Cv, &sh.C_[tr + t][n0]);
 #pragma unroll
@@ -312,7 +358,6 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                                 lam[c][j] = __fmul2_rn(l, da[t][c][j]);
                                 const float2 q = __fmul2_rn(lam[c][j], hh[t][c][j]);
                                 dBt[j] = c == 0 ? __fmul2_rn(l, du) : __ffma2_rn(l, du, dBt[j]);
-                                dCt[j] = c == 0 ? __fmul2_rn(go, hh[t + 1][c][j]) : __ffma2_rn(go, hh[t + 1][c][j], dCt[j]);
                                 r1 = j == 0 ? __fmul2_rn(l, Bv[j]) : __ffma2_rn(l, Bv[j], r1);
                                 r2 = j == 0 ? __fmul2_rn(q, A2[c][j]) : __ffma2_rn(q, A2[c][j], r2);
                                 dA[c][j] = __ffma2_rn(q, dt, dA[c][j]);
@@ -324,8 +369,6 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                         for (int j = 0; j < J; ++j) {
                             dB[2 * j][i] = dBt[j].x;
                             dB[2 * j + 1][i] = dBt[j].y;
-                            dC[2 * j][i] = dCt[j].x;
-                            dC[2 * j + 1][i] = dCt[j].y;
                         }
                     }
 #pragma unroll
@@ -333,19 +376,7 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                         keep(lb[c], &sh.lb[cl + c * CL][tr + tq]);
                         keep(qa[c], &sh.qa[cl + c * CL][tr + tq]);
                     }
-#pragma unroll
-                    for (int s = 0; s < S; ++s) {
-                        OverChannels::run(dB[s], lc);
-                        OverChannels::run(dC[s], lc);
-                    }
-                    if (OverChannels::stores(lc)) {
-#pragma unroll
-                        for (int i = 0; i < OverChannels::kHeld; ++i) {
-                            const int t = tr + tq + OverChannels::first(lc) + i;
-                            store_states<S>(&sh.red[warp][0][t][n0], dB, i);
-                            store_states<S>(&sh.red[warp][1][t][n0], dC, i);
-                        }
-                    }
+                    over_channels(dB, sh.red[warp][0], tq);
                 }
             }
             __syncthreads();
@@ -355,7 +386,7 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const int t = t_e + e * TS;
-                    if (t0 + t < p.T) {
+                    if (t0 + t < stop) {
                         const float2 u = unpack<IO, V>(&raw.u[t][ch]);
                         float2 go = unpack<IO, V>(&raw.g[t][ch]), gz = two(0.0f);
                         const float2 lb = make_float2(sh.lb[ch][t], sh.lb[ch + V - 1][t]);
@@ -403,7 +434,7 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                 }
             }
         }
-        if (g.grad_h0) put(g.grad_h0 + row, lam);
+        if (g.grad_h0 && split == 0) put(g.grad_h0 + row, lam);
         __syncthreads();                                        // before the next sequence's copies
     }
 
@@ -422,8 +453,124 @@ __global__ void __launch_bounds__(NT, 2) scan_bwd(const ScanParams p) {
                 e += sh.sums[1][i];
             }
             p.part_d[(long long)part * a.channels + chan + v] = d;
-            p.part_d[((long long)p.batch_parts + part) * a.channels + chan + v] = e;
+            p.part_d[((long long)parts + part) * a.channels + chan + v] = e;
         }
+    }
+}
+
+// What a part of a sequence (all but the first) adds to a_t l_t in front of it, from zero behind it,
+// and its sum of d: the walk of scan_bwd without anything else, for few long sequences.
+template <typename IO, int S, int SL>
+struct EndTile {
+    static constexpr int CL = 32 / SL, BC = NW * CL, NS = S * SL;
+    struct Raw {
+        IO d[TT][BC], z[TT][BC], g[TT][BC], C_[TT][NS];
+    };
+    __align__(16) Raw raw[2];
+    __align__(16) float C_[TT][NS];
+    float2 d[BC][TT + 1];                            // (d, grad o)
+};
+
+template <typename IO, int S, int SL, bool WIDE>
+__global__ void __launch_bounds__(NT) scan_bwd_ends(const ScanParams p) {
+    using Tl = EndTile<IO, S, SL>;
+    constexpr int CL = Tl::CL, BC = Tl::BC, NS = Tl::NS, J = S / 2;
+    constexpr int V = WIDE ? 2 : 1, ROW = BC / V;
+    constexpr int E = TT * ROW > NT ? TT * ROW / NT : 1, TS = TT / E;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Tl& sh = *reinterpret_cast<Tl*>(smem);
+    const dfsnn_state_scan_args& a = p.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    long long bid = blockIdx.x;
+    const int tile = (int)(bid % p.tiles);
+    bid /= p.tiles;
+    const int grp = (int)(bid % a.groups);
+    bid /= a.groups;
+    const int split = (int)(bid % (p.splits - 1)) + 1;
+    const long long b = bid / (p.splits - 1);
+    const int first = split * p.split_steps;
+    const int stop = p.T - first < p.split_steps ? p.T : first + p.split_steps;
+    const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T);
+    const int len = whole_len < stop ? whole_len : stop;
+    if (len <= first) return;
+    const int c_base = tile * BC, cols = p.group_channels - c_base;
+    const long long g_base = (long long)grp * p.group_channels;
+    const int ch = tid % ROW * V, t_e = tid / ROW;
+    const long long chan = g_base + c_base + ch;
+    float2 bias = two(0.0f);
+    if (ch < cols && a.delta_bias) bias = make_float2(a.delta_bias[chan], a.delta_bias[chan + V - 1]);
+    const int sl = lane / CL, cl = warp * CL + lane % CL, n0 = sl * S;
+    const long long ch_row = g_base + c_base + cl;
+    float2 A2[J], x[J] = {};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const bool ok = cl < cols;
+        A2[j].x = ok && n0 + 2 * j < a.states ? a.A[ch_row * a.states + n0 + 2 * j] * kLog2e : 0.0f;
+        A2[j].y = ok && n0 + 2 * j + 1 < a.states ? a.A[ch_row * a.states + n0 + 2 * j + 1] * kLog2e : 0.0f;
+    }
+    float steps = 0.0f;
+    auto fill = [&](int t0) {
+        const int rows = len - t0;
+        const long long c = g_base + c_base;
+        typename Tl::Raw& r = sh.raw[t0 / TT & 1];
+        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], static_cast<const IO*>(a.delta) + b * a.delta_b + c + t0 * a.delta_t, a.delta_t, rows, cols, p.words);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], static_cast<const IO*>(p.g.grad_y) + b * a.y_b + c + t0 * a.y_t, a.y_t, rows, cols, p.words);
+        if (a.z)
+            fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], static_cast<const IO*>(a.z) + b * a.z_b + c + t0 * a.z_t, a.z_t, rows, cols, p.words);
+        fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + t0 * a.C_t, a.C_t, rows, a.states, p.words);
+        copy_commit();
+    };
+    const int top = (len - 1) / TT * TT;
+    fill(top);
+    for (int t0 = top; t0 >= first; t0 -= TT) {
+        const typename Tl::Raw& raw = sh.raw[t0 / TT & 1];
+        copy_wait<0>();
+        __syncthreads();
+        if (t0 > first) fill(t0 - TT);
+        if (t_e < TT) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int t = t_e + e * TS;
+                float2 go = unpack<IO, V>(&raw.g[t][ch]), dt = __fadd2_rn(unpack<IO, V>(&raw.d[t][ch]), bias);
+                if (a.softplus) dt = softplus_f(dt);
+                if (t0 + t >= len) dt = two(0.0f);
+                if (a.z) {
+                    const float2 z = unpack<IO, V>(&raw.z[t][ch]);
+                    go = __fmul2_rn(go, __fmul2_rn(z, sigmoid_f(z)));
+                }
+                sh.d[ch][t] = make_float2(dt.x, go.x);
+                if (V == 2) sh.d[ch + V - 1][t] = make_float2(dt.y, go.y);
+            }
+        }
+#pragma unroll
+        for (int i = tid; i < TT * NS; i += NT) sh.C_[0][i] = to_f(raw.C_[0][i]);
+        __syncthreads();
+        float most = 0.0f;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) most = fmaxf(most, fabsf(sh.d[cl][t].x));
+        bool near1[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) near1[j] = most * fmaxf(fabsf(A2[j].x), fabsf(A2[j].y)) < kExp2Near;
+#pragma unroll
+        for (int t = TT - 1; t >= 0; --t) {
+            float2 Cv[J];
+            load_states<S>(Cv, &sh.C_[t][n0]);
+            const float2 d = sh.d[cl][t];
+            steps += d.x;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float2 y = __fmul2_rn(two(d.x), A2[j]), q = exp2_near1(y);
+                const float2 dec = make_float2(near1[j] ? q.x : exp2_approx(y.x), near1[j] ? q.y : exp2_approx(y.y));
+                x[j] = __fmul2_rn(dec, __ffma2_rn(Cv[j], two(d.y), x[j]));
+            }
+        }
+    }
+    if (cl < cols) {
+        const long long at = ((long long)split * a.batch + b) * a.channels + ch_row;
+        if (sl == 0) p.end_steps[at] = steps;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (n0 + s < a.states) p.ends[at * a.states + n0 + s] = s % 2 ? x[s / 2].y : x[s / 2].x;
     }
 }
 
@@ -434,6 +581,7 @@ __global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a)
     const dfsnn_state_scan_args& a = p.a;
     const dfsnn_state_scan_grads& g = p.g;
     const long long total = 2 * n_bc + n_a + 2 * a.channels;
+    const int parts = p.batch_parts * p.splits;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
          i += (long long)gridDim.x * blockDim.x) {
         float v = 0.0f;
@@ -447,7 +595,7 @@ __global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a)
             static_cast<IO*>(which ? g.grad_C : g.grad_B)[k] = from_f<IO>(v);
         } else if (i < 2 * n_bc + n_a) {
             const long long k = i - 2 * n_bc;
-            for (int j = 0; j < p.batch_parts; ++j) v += p.part_a[j * n_a + k];
+            for (int j = 0; j < parts; ++j) v += p.part_a[j * n_a + k];
             g.grad_A[k] = v;
         } else {
             const long long k = i - 2 * n_bc - n_a;
@@ -455,8 +603,8 @@ __global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a)
             float* out = which ? g.grad_delta_bias : g.grad_D;
             if (out) {
                 const long long c = k - which * a.channels;
-                for (int j = 0; j < p.batch_parts; ++j)
-                    v += p.part_d[((long long)which * p.batch_parts + j) * a.channels + c];
+                for (int j = 0; j < parts; ++j)
+                    v += p.part_d[((long long)which * parts + j) * a.channels + c];
                 out[c] = v;
             }
         }
@@ -465,8 +613,19 @@ __global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a)
 
 template <typename IO, int S, int SL, int C, bool WIDE>
 cudaError_t launch_form(const ScanParams& p, cudaStream_t st) {
-    const long long blocks = (long long)p.tiles * p.a.groups * p.batch_parts;
+    const long long blocks = (long long)p.tiles * p.a.groups * p.batch_parts * p.splits;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    if (p.splits > 1) {
+        using Ends = EndTile<IO, S, SL>;
+        ScanParams q = p;
+        q.tiles = (p.group_channels + Ends::BC - 1) / Ends::BC;
+        const long long n = (long long)q.tiles * p.a.groups * p.a.batch * (p.splits - 1);
+        if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
+        cudaError_t e = cudaFuncSetAttribute(scan_bwd_ends<IO, S, SL, WIDE>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Ends));
+        if (e != cudaSuccess) return e;
+        scan_bwd_ends<IO, S, SL, WIDE><<<(unsigned)n, NT, sizeof(Ends), st>>>(q);
+    }
     constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
     cudaError_t e = cudaFuncSetAttribute(scan_bwd<IO, S, SL, C, WIDE>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -492,10 +651,10 @@ cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     cudaError_t e;
     if (n <= 4) e = launch<IO, 2, 2, 1>(p, st);
     else if (n <= 8) e = launch<IO, 2, 4, 2>(p, st);
-    else if (n <= 16) e = launch<IO, 4, 4, 2>(p, st);
-    else if (n <= 32) e = launch<IO, 4, 8, 2>(p, st);
-    else if (n <= 64) e = launch<IO, 4, 16, 2>(p, st);
-    else e = launch<IO, 4, 32, 2>(p, st);
+    else if (n <= 16) e = launch<IO, 4, 4, 1>(p, st);
+    else if (n <= 32) e = launch<IO, 4, 8, 1>(p, st);
+    else if (n <= 64) e = launch<IO, 4, 16, 1>(p, st);
+    else e = launch<IO, 4, 32, 1>(p, st);
     if (e != cudaSuccess) return e;
     const long long n_bc = (long long)p.T * p.a.batch * p.a.groups * p.a.states;
     const long long n_a = p.a.channels * p.a.states;
@@ -509,10 +668,10 @@ cudaError_t pick(const ScanParams& p, cudaStream_t st) {
 int block_channels(int states) {
     if (states <= 4) return Tile<float, 2, 2, 1>::BC;
     if (states <= 8) return Tile<float, 2, 4, 2>::BC;
-    if (states <= 16) return Tile<float, 4, 4, 2>::BC;
-    if (states <= 32) return Tile<float, 4, 8, 2>::BC;
-    if (states <= 64) return Tile<float, 4, 16, 2>::BC;
-    return Tile<float, 4, 32, 2>::BC;
+    if (states <= 16) return Tile<float, 4, 4, 1>::BC;
+    if (states <= 32) return Tile<float, 4, 8, 1>::BC;
+    if (states <= 64) return Tile<float, 4, 16, 1>::BC;
+    return Tile<float, 4, 32, 1>::BC;
 }
 
 }  // namespace
@@ -522,12 +681,22 @@ int state_scan_bwd_tiles(int states, long long group_channels) {
     return (int)((group_channels + bc - 1) / bc);
 }
 
-// Blocks that share the batch: enough for 8 blocks an SM; beyond that each block takes several
+// How the blocks share sequences.  With few rows (blocks that walk whole sequences fill less than
+// half the machine) each sequence is cut into parts that run side by side, at the price of a second
+// walk for their ends.  With many, 8 blocks an SM are enough; beyond that a block takes several
 // sequences and adds its grad A on the way, which keeps the partial sums small.
-int state_scan_bwd_batch_parts(int states, long long batch, long long group_channels, int groups) {
-    const long long per = (long long)state_scan_bwd_tiles(states, group_channels) * groups;
-    const long long want = (148 * 8 + per - 1) / per;
-    return (int)std::max<long long>(1, std::min(batch, want));
+void state_scan_bwd_plan(ScanParams& p) {
+    const long long per = (long long)state_scan_bwd_tiles(p.a.states, p.group_channels) * p.a.groups;
+    const long long blocks = per * p.a.batch;
+    p.splits = 1;
+    p.split_steps = p.T;
+    p.batch_parts = (int)std::max<long long>(1, std::min(p.a.batch, (148 * 8 + per - 1) / per));
+    long long splits = std::min<long long>(148 * 3 / blocks, p.T / (8 * TT));
+    if (splits < 2) return;
+    const long long chunks = (p.T + TT - 1) / TT, each = (chunks + splits - 1) / splits;
+    p.split_steps = (int)(each * TT);
+    p.splits = (int)((chunks + each - 1) / each);
+    p.batch_parts = (int)p.a.batch;
 }
 
 cudaError_t state_scan_backward_launch(const ScanParams& p, cudaStream_t st) {

@@ -170,15 +170,15 @@ def test_scan_backward_refusals():
     f, size = L.dfsnn_state_scan_backward, L.dfsnn_state_scan_backward_workspace_size(32, 2, 8, 16, 1)
     assert size > 0 and L.dfsnn_state_scan_backward_workspace_size(0, 2, 8, 16, 1) == 0
     assert L.dfsnn_state_scan_backward_workspace_size(32, 2, 8, 16, 3) == 0
-    assert L.dfsnn_state_scan_kept_floats(32, 2, 8, 16) == 2 * 8 * 16
-    assert L.dfsnn_state_scan_kept_floats(16, 2, 8, 16) == 0
+    assert L.dfsnn_state_scan_kept_floats(32, 2, 8, 16) == (32 // _capi.SCAN_CHUNK - 1) * 2 * 8 * 16
+    assert L.dfsnn_state_scan_kept_floats(_capi.SCAN_CHUNK, 2, 8, 16) == 0
     full = [FAKE] * 11
     pack = lambda v: _capi.STATE_SCAN_GRADS.pack(*v, *([8] * 6))  # noqa: E731
     ws, E = ctypes.c_void_p(0x1000), _capi
     assert f(scan_pack(kept=FAKE), pack(full), None, size, None) == E.DFSNN_ERR_WORKSPACE
     assert f(scan_pack(kept=FAKE), pack(full), ctypes.c_void_p(0x1008), size, None) == E.DFSNN_ERR_WORKSPACE
     assert f(scan_pack(kept=FAKE), pack(full), ws, size - 1, None) == E.DFSNN_ERR_WORKSPACE
-    assert f(scan_pack(kept=0), pack(full), ws, size, None) == E.DFSNN_ERR_NULL     # T > 16 needs them
+    assert f(scan_pack(kept=0), pack(full), ws, size, None) == E.DFSNN_ERR_NULL     # long T needs them
     for i in (0, 2, 3, 5, 6, 7):                                                    # the required ones
         assert f(scan_pack(kept=FAKE), pack(full[:i] + [0] + full[i + 1:]), ws, size, None) == E.DFSNN_ERR_NULL
     assert f(scan_pack(kept=FAKE), None, ws, size, None) == E.DFSNN_ERR_NULL
