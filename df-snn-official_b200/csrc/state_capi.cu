@@ -55,8 +55,8 @@ dfsnn::ScanParams scan_params(const dfsnn_state_scan_args& a) {
 }
 
 struct ScanWorkspace {
-    size_t bc, a, d, ends, end_steps;       // floats
-    size_t bytes() const { return (bc + a + d + ends + end_steps) * sizeof(float); }
+    size_t bc, a, d, ends, end_steps, flags;       // 4-byte words
+    size_t bytes() const { return (bc + a + d + ends + end_steps + flags) * sizeof(float); }
 };
 
 ScanWorkspace backward_plan(dfsnn::ScanParams& p) {
@@ -68,7 +68,8 @@ ScanWorkspace backward_plan(dfsnn::ScanParams& p) {
     w.a = parts * p.a.channels * p.a.states;
     w.d = 2 * parts * p.a.channels;
     w.ends = p.splits > 1 ? p.splits * rows * p.a.states : 0;
-    w.end_steps = p.splits > 1 ? p.splits * rows : 0;
+    w.end_steps = p.splits > 1 && !p.chained ? p.splits * rows : 0;
+    w.flags = p.chained ? (size_t)p.tiles * p.a.groups * p.batch_parts + 1 : 0;
     return w;
 }
 
@@ -139,6 +140,8 @@ int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_
     p.part_d = p.part_a + w.a;
     p.ends = p.part_d + w.d;
     p.end_steps = p.ends + w.ends;
+    p.flags = reinterpret_cast<int*>(p.end_steps + w.end_steps);
+    p.error = p.flags + (w.flags ? w.flags - 1 : 0);
     return status(dfsnn::state_scan_backward_launch(p, (cudaStream_t)stream));
 }
 

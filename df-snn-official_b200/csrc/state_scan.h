@@ -17,6 +17,9 @@ struct ScanParams {
     int splits, split_steps;
     float* ends;                               // [splits][batch][channels][states] (forward: all but
     float* end_steps;                          // the last, backward: the first unused) and sums of d
+    int chained;                               // backward: the parts run in order, `ends` passed on
+    int* flags;                                // [tiles * groups * batch] finished parts, zeroed first
+    int* error;                                // behind them: a wait that ran out
     // backward
     int batch_parts;                           // blocks that share the batch (part q: b = q, q + parts, ...)
     float* part_bc;                            // [2][tiles][T][batch][groups][states]

@@ -42,6 +42,7 @@ struct Tile {
     float g[BC][TT + 1];                             // grad o
     float lb[BC][TT + 1], qa[BC][TT + 1], o[BC][TT + 1];    // sums over states
     float sums[2][NT];
+    int ready;
 };
 
 template <int S>
@@ -79,6 +80,23 @@ __device__ __forceinline__ void store(IO* q, float2 f) {
     *reinterpret_cast<Pack<IO, V>*>(q) = p;
 }
 
+// The flag of a chain counts its finished parts.  A wait ends after some seconds at the latest: then
+// the error word is set and the caller goes on with NaN, which reaches all that depends on it.
+constexpr unsigned kMaxPolls = 1u << 21;
+__device__ __forceinline__ bool wait_at_least(const int* flag, int count, int* error) {
+    for (unsigned i = 0; i < kMaxPolls; ++i) {
+        int v;
+        asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+        if (v >= count) return true;
+        __nanosleep(200);
+    }
+    *error = 1;
+    return false;
+}
+__device__ __forceinline__ void publish(int* flag, int count) {
+    asm volatile("st.release.gpu.global.b32 [%0], %1;" ::"l"(flag), "r"(count) : "memory");
+}
+
 template <typename IO, int S, int SL, int C, bool WIDE>
 __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
     using Tl = Tile<IO, S, SL, C>;
@@ -94,11 +112,22 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     long long bid = blockIdx.x;
+    const long long chains = (long long)p.tiles * a.groups * p.batch_parts;
+    const long long chain = p.chained ? bid % chains : 0;       // (tile, group, sequence)
+    int split = 0;
+    if (p.chained) {                                            // all last parts, then all last but one, ...
+        split = p.splits - 1 - (int)(bid / chains);
+        bid = chain;
+    }
     const int tile = (int)(bid % p.tiles);
     bid /= p.tiles;
     const int grp = (int)(bid % a.groups);
     bid /= a.groups;
-    const int split = (int)(bid % p.splits), batch_part = (int)(bid / p.splits);
+    if (!p.chained) {
+        split = (int)(bid % p.splits);
+        bid /= p.splits;
+    }
+    const int batch_part = (int)bid;
     const int first = split * p.split_steps;                    // this part's steps: first .. stop - 1
     const int stop = p.T - first < p.split_steps ? p.T : first + p.split_steps;
     const int part = batch_part * p.splits + split, parts = p.batch_parts * p.splits;
@@ -193,10 +222,21 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
         float2 start[C][J] = {};                                // loaded one chunk ahead
         if (top >= 0) state_at((len - 1) / R * R, start);
         float2 lam[C][J] = {};                                  // a_(t+1) l_(t+1)
-        if (len > first || split == 0) {
+        const long long rows = a.batch * a.channels;
+        if (p.chained && len > first && whole_len > stop) {
+            // the part behind this one: its block has a lower index, so it runs or has run
+            if (tid == 0) sh.ready = wait_at_least(p.flags + chain, p.splits - 1 - split, p.error);
+            __syncthreads();
+            get(p.ends + split * rows * a.states + row, lam);
+            if (!sh.ready) {
+#pragma unroll
+                for (int c = 0; c < C; ++c)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) lam[c][j] = two(__int_as_float(0x7fc00000));
+            }
+        } else if (len > first || split == 0) {
             get(g.grad_h_last ? g.grad_h_last + row : nullptr, lam);
-            const long long rows = a.batch * a.channels;
-            for (int k = (whole_len - 1) / p.split_steps; k > split; --k) {
+            if (!p.chained) for (int k = (whole_len - 1) / p.split_steps; k > split; --k) {
                 float2 end[C][J] = {};
                 get(p.ends + k * rows * a.states + row, end);
 #pragma unroll
@@ -435,6 +475,12 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
             }
         }
         if (g.grad_h0 && split == 0) put(g.grad_h0 + row, lam);
+        if (p.chained && split > 0 && len > first) {            // for the part in front
+            put(p.ends + (split - 1) * rows * a.states + row, lam);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) publish(p.flags + chain, p.splits - split);
+        }
         __syncthreads();                                        // before the next sequence's copies
     }
 
@@ -574,40 +620,61 @@ __global__ void __launch_bounds__(NT) scan_bwd_ends(const ScanParams p) {
     }
 }
 
-// Adds the blocks' parts: grad B and grad C over the channel tiles, then grad A, D and delta_bias
-// over the batch parts, one thread for an output, in order.
+// Adds the blocks' parts in a fixed order.  Blocks 0 .. bc_blocks - 1: grad B and grad C over the
+// channel tiles, a thread for an output.  The others: grad A, D and delta_bias over the parts of
+// the batch and the sequences, 32 outputs a block; its 8 warps add every eighth part, then the
+// warps' sums are added in order.
+constexpr int kSumThreads = 256;
 template <typename IO>
-__global__ void scan_bwd_sums(const ScanParams p, long long n_bc, long long n_a) {
+__global__ void __launch_bounds__(kSumThreads) scan_bwd_sums(const ScanParams p, int bc_blocks) {
     const dfsnn_state_scan_args& a = p.a;
     const dfsnn_state_scan_grads& g = p.g;
-    const long long total = 2 * n_bc + n_a + 2 * a.channels;
-    const int parts = p.batch_parts * p.splits;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-         i += (long long)gridDim.x * blockDim.x) {
-        float v = 0.0f;
-        if (i < 2 * n_bc) {
+    const long long n_bc = (long long)p.T * a.batch * a.groups * a.states;
+    const long long n_a = a.channels * a.states;
+    if (blockIdx.x < bc_blocks) {
+        for (long long i = (long long)blockIdx.x * kSumThreads + threadIdx.x; i < 2 * n_bc;
+             i += (long long)bc_blocks * kSumThreads) {
+            float v = 0.0f;
             const int which = i >= n_bc;
-            const long long k = i - which * n_bc, row = k / ((long long)a.groups * a.states);
+            const long long k = i - which * n_bc, row = k / (a.groups * a.states);
             if (row / a.batch < seq_length(a.lengths, a.lengths64, row % a.batch, p.T)) {
                 const float* q = p.part_bc + (long long)which * p.tiles * n_bc + k;
+#pragma unroll 4
                 for (int j = 0; j < p.tiles; ++j) v += q[j * n_bc];
             }
             static_cast<IO*>(which ? g.grad_C : g.grad_B)[k] = from_f<IO>(v);
-        } else if (i < 2 * n_bc + n_a) {
-            const long long k = i - 2 * n_bc;
-            for (int j = 0; j < parts; ++j) v += p.part_a[j * n_a + k];
-            g.grad_A[k] = v;
-        } else {
-            const long long k = i - 2 * n_bc - n_a;
-            const int which = k >= a.channels;
-            float* out = which ? g.grad_delta_bias : g.grad_D;
-            if (out) {
-                const long long c = k - which * a.channels;
-                for (int j = 0; j < parts; ++j)
-                    v += p.part_d[((long long)which * parts + j) * a.channels + c];
-                out[c] = v;
-            }
         }
+        return;
+    }
+    __shared__ float s_sum[kSumThreads / 32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long i = (long long)(blockIdx.x - bc_blocks) * 32 + lane;
+    const int parts = p.batch_parts * p.splits;
+    const float* q = nullptr;
+    long long stride = n_a;
+    float* out = nullptr;
+    if (i < n_a) {
+        q = p.part_a + i;
+        out = g.grad_A + i;
+    } else if (i < n_a + 2 * a.channels) {
+        const int which = i - n_a >= a.channels;
+        const long long c = i - n_a - which * a.channels;
+        stride = a.channels;
+        q = p.part_d + which * parts * a.channels + c;
+        out = which ? g.grad_delta_bias : g.grad_D;
+        if (out) out += c;
+    }
+    float v = 0.0f;
+    if (out) {
+#pragma unroll 4
+        for (int j = warp; j < parts; j += kSumThreads / 32) v += q[j * stride];
+    }
+    s_sum[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && out) {
+        v = 0.0f;
+        for (int w = 0; w < kSumThreads / 32; ++w) v += s_sum[w][lane];
+        *out = v;
     }
 }
 
@@ -615,7 +682,10 @@ template <typename IO, int S, int SL, int C, bool WIDE>
 cudaError_t launch_form(const ScanParams& p, cudaStream_t st) {
     const long long blocks = (long long)p.tiles * p.a.groups * p.batch_parts * p.splits;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    if (p.splits > 1) {
+    if (p.chained) {
+        const cudaError_t e = cudaMemsetAsync(p.flags, 0, (p.tiles * p.a.groups * p.batch_parts + 1) * sizeof(int), st);
+        if (e != cudaSuccess) return e;
+    } else if (p.splits > 1) {
         using Ends = EndTile<IO, S, SL>;
         ScanParams q = p;
         q.tiles = (p.group_channels + Ends::BC - 1) / Ends::BC;
@@ -657,10 +727,9 @@ cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     else e = launch<IO, 4, 32, 1>(p, st);
     if (e != cudaSuccess) return e;
     const long long n_bc = (long long)p.T * p.a.batch * p.a.groups * p.a.states;
-    const long long n_a = p.a.channels * p.a.states;
-    const long long total = 2 * n_bc + n_a + 2 * p.a.channels;
-    const unsigned blocks = (unsigned)std::min<long long>((total + 255) / 256, 148 * 16);
-    scan_bwd_sums<IO><<<blocks, 256, 0, st>>>(p, n_bc, n_a);
+    const int bc_blocks = (int)std::min<long long>((2 * n_bc + kSumThreads - 1) / kSumThreads, 148 * 16);
+    const long long params = (p.a.channels * (p.a.states + 2) + 31) / 32;
+    scan_bwd_sums<IO><<<(unsigned)(bc_blocks + params), kSumThreads, 0, st>>>(p, bc_blocks);
     return cudaGetLastError();
 }
 
@@ -683,7 +752,10 @@ int state_scan_bwd_tiles(int states, long long group_channels) {
 
 // How the blocks share sequences.  With few rows (blocks that walk whole sequences fill less than
 // half the machine) each sequence is cut into parts that run side by side, at the price of a second
-// walk for their ends.  With many, 8 blocks an SM are enough; beyond that a block takes several
+// walk for their ends.  With somewhat more blocks than run at a time, the last round would leave
+// most of the machine idle for a whole walk; the sequences are then cut into parts that run one
+// after another, a block passing its a_t l_t on to the next (chained), so that the last round is a
+// short one.  With many, 8 blocks an SM are enough; beyond that a block takes several
 // sequences and adds its grad A on the way, which keeps the partial sums small.
 void state_scan_bwd_plan(ScanParams& p) {
     const long long per = (long long)state_scan_bwd_tiles(p.a.states, p.group_channels) * p.a.groups;
@@ -691,7 +763,13 @@ void state_scan_bwd_plan(ScanParams& p) {
     p.splits = 1;
     p.split_steps = p.T;
     p.batch_parts = (int)std::max<long long>(1, std::min(p.a.batch, (148 * 8 + per - 1) / per));
-    long long splits = std::min<long long>(148 * 3 / blocks, p.T / (8 * TT));
+    p.chained = 0;
+    const long long slots = 148 * 3;                    // blocks that run at a time
+    long long splits = std::min<long long>(slots / blocks, p.T / (8 * TT));
+    if (splits < 2 && blocks > slots) {
+        splits = std::min<long long>(8 * slots / blocks, p.T / (8 * TT));
+        p.chained = splits > 1;
+    }
     if (splits < 2) return;
     const long long chunks = (p.T + TT - 1) / TT, each = (chunks + splits - 1) / splits;
     p.split_steps = (int)(each * TT);

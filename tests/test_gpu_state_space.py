@@ -118,6 +118,16 @@ def test_scan_batch_first_views():
     assert torch.autograd.grad(y.float().sum(), u)[0].shape == u.shape
 
 
+@pytest.mark.parametrize("T,B,D,N,G,lengths", [
+    (300, 480, 8, 16, 1, None), (270, 64, 250, 12, 2, "ragged"), (290, 300, 33, 4, 1, "ragged")])
+def test_scan_backward_in_rounds(T, B, D, N, G, lengths):
+    """More blocks than run at a time: the parts of a sequence run one after another."""
+    if lengths:
+        lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(T)).tolist()
+    x, n, grads = scan_case(T, B, D, N, G, "f32", lengths=lengths, seed=T, scale=0.1)
+    check_scan(x, n, grads, True, f"rounds {T}x{B}x{D}")
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("shift", [0, 1, 2, 4])
 @pytest.mark.parametrize("D,N,G", [(64, 16, 1), (66, 12, 2), (33, 7, 1), (24, 100, 1), (8, 3, 1)])
