@@ -38,7 +38,8 @@ _ACTIVATIONS = (None, "silu")
 
 
 # ---------------------------------------------------------------------------------------
-# argument checks
+# argument checks.  They run on every call of a token loop, so each is one comparison for a good
+# argument; what is wrong with a bad one is worked out afterwards.
 # ---------------------------------------------------------------------------------------
 def _lead(x, name, dims):
     """The sequence that sets a call's shape, type and device."""
@@ -48,55 +49,52 @@ def _lead(x, name, dims):
         raise ValueError(f"{name}: float32, float16 or bfloat16 sequences, got {x.dtype}")
     if x.dim() != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got {tuple(x.shape)}")
-    return _rows(x)
+    return x if x.stride(-1) == 1 else _rows(x)
 
 
 def _rows(x):
     return x if x.stride(-1) == 1 or x.size(-1) == 1 else x.contiguous()
 
 
-def _seq(x, like, shape, name, what):
+def _seq(x, dtype, dev, shape, name, what):
     """A further sequence of the call: same type and device, given shape, unit last stride."""
-    if x.dtype != like.dtype or x.device != like.device:
-        raise ValueError(f"{name}: {what} must be {like.dtype} on {like.device}, got {x.dtype} on {x.device}")
-    if x.shape != shape:
-        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(x.shape)}")
-    return _rows(x)
+    if x.dtype is not dtype or x.get_device() != dev or x.shape != shape:
+        raise ValueError(f"{name}: {what} must be {dtype} {tuple(shape)} on cuda:{dev}, got {x.dtype} "
+                         f"{tuple(x.shape)} on {x.device}")
+    return x if x.stride(-1) == 1 else _rows(x)
 
 
-def _param(x, device, shape, name, what):
+def _param(x, dev, shape, name, what):
     """A float32 parameter or state (converted if need be), dense."""
     if x is None:
         return None
-    if x.device != device:
-        raise ValueError(f"{name}: {what} must be on {device}, got {x.device}")
-    if x.shape != shape:
-        raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(x.shape)}")
-    if not x.dtype.is_floating_point:
-        raise ValueError(f"{name}: {what} must be floating-point, got {x.dtype}")
-    return (x if x.dtype == torch.float32 else x.float()).contiguous()
+    if x.get_device() != dev or x.shape != shape or not x.dtype.is_floating_point:
+        raise ValueError(f"{name}: {what} must be floating-point {tuple(shape)} on cuda:{dev}, got "
+                         f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    if x.dtype is not torch.float32:
+        x = x.float()
+    return x if x.is_contiguous() else x.contiguous()
 
 
-def _integers(x, device, count, name, what):
+def _integers(x, dev, count, name, what):
     if x is None:
         return None
-    if x.dtype not in (torch.int32, torch.int64) or x.shape != (count,) or x.device != device:
-        raise ValueError(f"{name}: {what} must be int32 or int64 [{count}] on {device}, got "
+    if x.dtype not in (torch.int32, torch.int64) or x.shape != (count,) or x.get_device() != dev:
+        raise ValueError(f"{name}: {what} must be int32 or int64 [{count}] on cuda:{dev}, got "
                          f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
-def _groups(x, like, lead, name, what):
+def _groups(x, dtype, dev, lead, name, what):
     """B or C as [..., G, N]; [..., N] is one group."""
     if x.dim() == len(lead) + 1:
         x = x.unsqueeze(-2)
     if x.dim() != len(lead) + 2:
         raise ValueError(f"{name}: {what} must be {tuple(lead)} + ([groups,] states), got {tuple(x.shape)}")
-    return _seq(x, like, (*lead, *x.shape[-2:]), name, what)
+    return _seq(x, dtype, dev, (*lead, *x.shape[-2:]), name, what)
 
 
-def _scan_sizes(u, A, B, C, name):
-    D = u.shape[-1]
+def _scan_sizes(D, A, B, C, name):
     if A.dim() != 2 or A.shape[0] != D:
         raise ValueError(f"{name}: A must have shape ({D}, states), got {tuple(A.shape)}")
     N, G = A.shape[1], B.shape[-2]
@@ -107,7 +105,7 @@ def _scan_sizes(u, A, B, C, name):
         raise ValueError(f"{name}: 1 to {_capi.SCAN_MAX_STATES} states, got {N}")
     if G < 1 or D % G:
         raise ValueError(f"{name}: {D} channels do not divide into {G} groups")
-    return D, N, G
+    return N, G
 
 
 def _taps(weight, D, name):
@@ -125,48 +123,62 @@ def _silu_flag(activation, name):
     return int(activation == "silu")
 
 
-def _pool(state, state_out, device, dtype, inner, rows, index, name):
-    """(state, state_out, slots) of a step call.  Slots may lie anywhere along dimension 0 (one
-    layer of a pool for several), but each is dense: they are written in place."""
-    if state_out is None:
-        state_out = state
-    dense = (inner[1], 1)
-    for x, what in ((state, "state"), (state_out, "state_out")):
-        if x.dtype != dtype or x.device != device or x.dim() != 3 or x.shape[1:] != inner:
-            raise ValueError(f"{name}: {what} must be {dtype} [slots, {inner[0]}, {inner[1]}] on "
-                             f"{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-        if x.numel() and x.stride()[1:] != dense and x.shape[1:] != (1, 1):
-            raise ValueError(f"{name}: each slot of {what} must be contiguous")
-        if x.shape[0] > 1 and x.stride(0) < inner[0] * inner[1]:
-            raise ValueError(f"{name}: the slots of {what} overlap")
-        if x.requires_grad:
-            raise ValueError(f"{name}: {what} is written in place and cannot require a gradient")
-    slots = state.shape[0]
-    if state_out.shape[0] != slots:
-        raise ValueError(f"{name}: state_out must have {slots} slots, got {state_out.shape[0]}")
+def _slots(x, dtype, dev, inner, name, what):
+    """Checks a pool of states [slots, *inner] and returns (slots, stride).  Slots may lie anywhere
+    along dimension 0 (one layer of a pool for several), but each is dense: they are written in
+    place."""
+    if x.dtype is not dtype or x.get_device() != dev or x.dim() != 3 or x.shape[1:] != inner:
+        raise ValueError(f"{name}: {what} must be {dtype} [slots, {inner[0]}, {inner[1]}] on cuda:{dev}, "
+                         f"got {x.dtype} {tuple(x.shape)} on {x.device}")
+    stride = x.stride()
+    if stride[1:] != (inner[1], 1) and x.numel() and x.shape[1:] != (1, 1):
+        raise ValueError(f"{name}: each slot of {what} must be contiguous")
+    if stride[0] < inner[0] * inner[1] and x.shape[0] > 1:
+        raise ValueError(f"{name}: the slots of {what} overlap")
+    if x.requires_grad:
+        raise ValueError(f"{name}: {what} is written in place and cannot require a gradient")
+    return x.shape[0], stride[0]
+
+
+def _pool(state, state_out, dtype, dev, inner, rows, index, name):
+    """(state_out, slots, strides) of a step call."""
+    slots, stride = _slots(state, dtype, dev, inner, name, "state")
+    if state_out is None or state_out is state:
+        state_out, out_stride = state, stride
+    else:
+        out_slots, out_stride = _slots(state_out, dtype, dev, inner, name, "state_out")
+        if out_slots != slots:
+            raise ValueError(f"{name}: state_out must have {slots} slots, got {out_slots}")
     if index is None and slots < rows:
         raise ValueError(f"{name}: {rows} rows need as many slots, got {slots}")
     if torch.is_grad_enabled() and not state_out.is_inference():
         torch.autograd.graph.increment_version(state_out)
-    return state, state_out, slots
+    return state_out, slots, stride, out_stride
 
 
 # ---------------------------------------------------------------------------------------
 # calls
 # ---------------------------------------------------------------------------------------
-def _call(fn, name, launches, nbytes, device, *args):
-    """One native call on the current stream of `device`."""
-    if device.index != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return _call(fn, name, launches, nbytes, device, *args)
-    stream = torch.cuda.current_stream(device).cuda_stream
+def _call(fn, name, launches, nbytes, dev, *args):
+    """One native call on the current stream of device number `dev`."""
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _call(fn, name, launches, nbytes, dev, *args)
     if _prof._ACTIVE is None:
-        code = fn(*args, stream)
+        code = fn(*args, _raw_stream(dev))
     else:
-        with _prof.native_call(name, launches, nbytes(), device):
-            code = fn(*args, stream)
+        with _prof.native_call(name, launches, nbytes(), torch.device("cuda", dev)):
+            code = fn(*args, _raw_stream(dev))
     if code:
         _capi.check(code, name)
+
+
+def _raw_stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream    # the same number without a Stream object
 
 
 def _p(t):
@@ -174,43 +186,39 @@ def _p(t):
 
 
 def _tb(t):
-    return (0, 0) if t is None else (t.stride(0), t.stride(1))
+    return (0, 0) if t is None else t.stride()[:2]
 
 
-def _empty_like(x, zero=False):
-    """[T, B, D], dense, batch-first in memory where x is."""
-    T, B, D = x.shape
-    make = torch.zeros if zero else torch.empty
-    if T > 1 and B > 1 and x.stride(1) > x.stride(0):
-        return make((B, T, D), dtype=x.dtype, device=x.device).transpose(0, 1)
-    return make((T, B, D), dtype=x.dtype, device=x.device)
+def _empty_like(x):
+    """Dense, in the order of x (batch-first in memory where x is), with unit last stride."""
+    y = torch.empty_like(x)
+    if y.stride(-1) != 1 and y.size(-1) != 1:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    return y
 
 
 def _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, y_strides, h_last, kept):
     T, Bn, Dn = u.shape
     return _capi.STATE_SCAN_ARGS.pack(
-        _p(u), _p(delta), _p(z), _p(B), _p(C), _p(A), _p(D), _p(bias), _p(h0), _p(lengths), _p(y),
-        _p(h_last), _p(kept), *_tb(u), *_tb(delta), *_tb(z), *B.stride()[:3], *C.stride()[:3],
-        *y_strides, T, Bn, Dn, A.shape[1], B.shape[2], _DTYPES[u.dtype], int(softplus),
-        int(lengths is not None and lengths.dtype == torch.int64), 0)
+        u.data_ptr(), delta.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(bias),
+        _p(h0), _p(lengths), _p(y), _p(h_last), _p(kept), *u.stride()[:2], *delta.stride()[:2], *_tb(z),
+        *B.stride()[:3], *C.stride()[:3], *y_strides, T, Bn, Dn, A.shape[1], B.shape[2], _DTYPES[u.dtype],
+        int(softplus), int(lengths is not None and lengths.dtype is torch.int64), 0)
 
 
 def _scan_forward(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, want_last, keep):
     T, Bn, Dn = u.shape
-    N = A.shape[1]
+    N, dev = A.shape[1], u.get_device()
     lib = _capi.lib()
     y = _empty_like(u)
-    h_last = torch.empty((Bn, Dn, N), dtype=torch.float32, device=u.device) if want_last else None
-    kept = None
-    if keep:
-        count = lib.dfsnn_state_scan_kept_floats(T, Bn, Dn, N)
-        kept = torch.empty(count, dtype=torch.float32, device=u.device)
-    args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, _tb(y), h_last, kept)
+    h_last = A.new_empty((Bn, Dn, N)) if want_last else None
+    kept = A.new_empty(lib.dfsnn_state_scan_kept_floats(T, Bn, Dn, N)) if keep else None
+    args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, softplus, y, y.stride()[:2], h_last, kept)
     size = lib.dfsnn_state_scan_forward_workspace_size(T, Bn, Dn, N, B.shape[2])
-    ws = torch.empty(size, dtype=torch.uint8, device=u.device) if size else None
+    ws = A.new_empty(size // 4) if size else None
     _call(lib.dfsnn_state_scan_forward, "state_scan_forward", 2 if size else 1,
           lambda: _prof.state_scan_bytes(T, Bn, Dn, N, B.shape[2], u.element_size(), z is not None, False),
-          u.device, args, _p(ws), size)
+          dev, args, _p(ws), size)
     return y, h_last, kept
 
 
@@ -233,26 +241,26 @@ class StateScanFunction(torch.autograd.Function):
         u, delta, A, B, C, D, z, bias, h0, lengths, kept = ctx.saved_tensors
         T, Bn, Dn = u.shape
         N, G = A.shape[1], B.shape[2]
-        dev, empty = u.device, Bn == 0 or Dn == 0
-        gy = _empty_like(u, zero=True) if grad_y is None else _rows(grad_y)
-        gl = None if grad_last is None else grad_last.float().contiguous()
+        gy = torch.zeros_like(u) if grad_y is None else grad_y
+        gy = gy if gy.stride(-1) == 1 else _rows(gy)
+        gl = None if grad_last is None else grad_last.contiguous()
         gu, gdelta = _empty_like(u), _empty_like(delta)
         gz = None if z is None else _empty_like(z)
-        gB, gC = (torch.empty((T, Bn, G, N), dtype=u.dtype, device=dev) for _ in range(2))
-        make = torch.zeros_like if empty else torch.empty_like
+        gB, gC = u.new_empty((T, Bn, G, N)), u.new_empty((T, Bn, G, N))
+        make = torch.zeros_like if Bn == 0 or Dn == 0 else torch.empty_like
         gA = make(A)
         gD, gbias, gh0 = (None if x is None else make(x) for x in (D, bias, h0))
         lib = _capi.lib()
-        args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, ctx.softplus, None, _tb(gy),
+        args = _scan_args(u, delta, A, B, C, D, z, bias, h0, lengths, ctx.softplus, None, gy.stride()[:2],
                           None, kept)
         grads = _capi.STATE_SCAN_GRADS.pack(
-            _p(gy), _p(gl), _p(gu), _p(gdelta), _p(gz), _p(gB), _p(gC), _p(gA), _p(gD), _p(gbias),
-            _p(gh0), *_tb(gu), *_tb(gdelta), *_tb(gz))
+            gy.data_ptr(), _p(gl), gu.data_ptr(), gdelta.data_ptr(), _p(gz), gB.data_ptr(), gC.data_ptr(),
+            gA.data_ptr(), _p(gD), _p(gbias), _p(gh0), *gu.stride()[:2], *gdelta.stride()[:2], *_tb(gz))
         size = lib.dfsnn_state_scan_backward_workspace_size(T, Bn, Dn, N, G)
-        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        ws = A.new_empty(size // 4)
         _call(lib.dfsnn_state_scan_backward, "state_scan_backward", 2,
               lambda: _prof.state_scan_bytes(T, Bn, Dn, N, G, u.element_size(), z is not None, True),
-              dev, args, grads, ws.data_ptr(), ws.numel())
+              u.get_device(), args, grads, ws.data_ptr(), size)
         return gu, gdelta, gA, gB, gC, gD, gz, gbias, gh0, None, None, None
 
 
@@ -269,18 +277,20 @@ def state_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=Fals
     also the states after each sequence's last step, float32 [B, D, N]."""
     name = "state_scan"
     u = _lead(u, name, 3)
-    T, Bn, Dn = u.shape
+    shape, dtype, dev = u.shape, u.dtype, u.get_device()
+    T, Bn, Dn = shape
     if T < 1:
         raise ValueError(f"{name}: at least one step, got T = {T}")
-    delta = _seq(delta, u, u.shape, name, "delta")
-    z = None if z is None else _seq(z, u, u.shape, name, "z")
-    B, C = _groups(B, u, (T, Bn), name, "B"), _groups(C, u, (T, Bn), name, "C")
-    _, N, _ = _scan_sizes(u, A, B, C, name)
-    A = _param(A, u.device, (Dn, N), name, "A")
-    D = _param(D, u.device, (Dn,), name, "D")
-    bias = _param(delta_bias, u.device, (Dn,), name, "delta_bias")
-    h0 = _param(h0, u.device, (Bn, Dn, N), name, "h0")
-    lengths = _integers(lengths, u.device, Bn, name, "lengths")
+    delta = _seq(delta, dtype, dev, shape, name, "delta")
+    if z is not None:
+        z = _seq(z, dtype, dev, shape, name, "z")
+    B, C = _groups(B, dtype, dev, (T, Bn), name, "B"), _groups(C, dtype, dev, (T, Bn), name, "C")
+    N, _ = _scan_sizes(Dn, A, B, C, name)
+    A = _param(A, dev, (Dn, N), name, "A")
+    D = _param(D, dev, (Dn,), name, "D")
+    bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
+    h0 = _param(h0, dev, (Bn, Dn, N), name, "h0")
+    lengths = _integers(lengths, dev, Bn, name, "lengths")
     tensors = (u, delta, A, B, C, D, z, bias, h0)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         y, last = StateScanFunction.apply(*tensors, lengths, bool(softplus), bool(return_state))
@@ -301,24 +311,24 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
     y [B, D]."""
     name = "state_scan_step"
     u = _lead(u, name, 2)
-    Bn, Dn = u.shape
-    delta = _seq(delta, u, u.shape, name, "delta")
-    z = None if z is None else _seq(z, u, u.shape, name, "z")
-    B, C = _groups(B, u, (Bn,), name, "B"), _groups(C, u, (Bn,), name, "C")
-    _, N, G = _scan_sizes(u, A, B, C, name)
-    dev = u.device
+    shape, dtype, dev = u.shape, u.dtype, u.get_device()
+    Bn, Dn = shape
+    delta = _seq(delta, dtype, dev, shape, name, "delta")
+    if z is not None:
+        z = _seq(z, dtype, dev, shape, name, "z")
+    B, C = _groups(B, dtype, dev, (Bn,), name, "B"), _groups(C, dtype, dev, (Bn,), name, "C")
+    N, G = _scan_sizes(Dn, A, B, C, name)
     A = _param(A, dev, (Dn, N), name, "A")
     D = _param(D, dev, (Dn,), name, "D")
     bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
     index = _integers(index, dev, Bn, name, "index")
-    state, state_out, slots = _pool(state, state_out, dev, torch.float32, (Dn, N), Bn, index, name)
-    y = torch.empty((Bn, Dn), dtype=u.dtype, device=dev)
+    state_out, slots, s_in, s_out = _pool(state, state_out, torch.float32, dev, (Dn, N), Bn, index, name)
+    y = u.new_empty(shape)
     args = _capi.STATE_SCAN_STEP_ARGS.pack(
-        _p(u), _p(delta), _p(z), _p(B), _p(C), _p(A), _p(D), _p(bias), _p(state), _p(state_out),
-        _p(index), _p(y), u.stride(0), delta.stride(0), 0 if z is None else z.stride(0),
-        B.stride(0), B.stride(1), C.stride(0), C.stride(1), Dn, state.stride(0),
-        state_out.stride(0), Bn, Dn, slots, N, G, _DTYPES[u.dtype], int(softplus),
-        int(index is not None and index.dtype == torch.int64), 0)
+        u.data_ptr(), delta.data_ptr(), _p(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), _p(D), _p(bias),
+        state.data_ptr(), state_out.data_ptr(), _p(index), y.data_ptr(), u.stride(0), delta.stride(0),
+        0 if z is None else z.stride(0), *B.stride()[:2], *C.stride()[:2], Dn, s_in, s_out, Bn, Dn, slots,
+        N, G, _DTYPES[dtype], int(softplus), int(index is not None and index.dtype is torch.int64), 0)
     _call(_capi.lib().dfsnn_state_scan_step, name, 1,
           lambda: _prof.state_scan_step_bytes(Bn, Dn, N, G, u.element_size(), z is not None), dev, args)
     return y
@@ -327,19 +337,19 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
 def _conv_args(x, weight, bias, state, lengths, silu, y, y_strides, last):
     T, Bn, Dn = x.shape
     return _capi.SHORT_CONV_ARGS.pack(
-        _p(x), _p(weight), _p(bias), _p(state), _p(lengths), _p(y), _p(last), *_tb(x), *y_strides,
-        T, Bn, Dn, weight.shape[1], _DTYPES[x.dtype], silu,
-        int(lengths is not None and lengths.dtype == torch.int64))
+        x.data_ptr(), weight.data_ptr(), _p(bias), _p(state), _p(lengths), _p(y), _p(last), *x.stride()[:2],
+        *y_strides, T, Bn, Dn, weight.shape[1], _DTYPES[x.dtype], silu,
+        int(lengths is not None and lengths.dtype is torch.int64))
 
 
 def _conv_forward(x, weight, bias, state, lengths, silu, want_last):
     T, Bn, Dn = x.shape
     W = weight.shape[1]
     y = _empty_like(x)
-    last = torch.empty((Bn, W - 1, Dn), dtype=x.dtype, device=x.device) if want_last else None
-    args = _conv_args(x, weight, bias, state, lengths, silu, y, _tb(y), last)
+    last = x.new_empty((Bn, W - 1, Dn)) if want_last else None
+    args = _conv_args(x, weight, bias, state, lengths, silu, y, y.stride()[:2], last)
     _call(_capi.lib().dfsnn_short_conv_forward, "short_conv_forward", 1,
-          lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), False), x.device, args)
+          lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), False), x.get_device(), args)
     return y, last
 
 
@@ -360,21 +370,23 @@ class ShortConvFunction(torch.autograd.Function):
     def backward(ctx, grad_y, grad_last):
         x, weight, bias, state, lengths = ctx.saved_tensors
         T, Bn, Dn = x.shape
-        W, dev = weight.shape[1], x.device
-        gy = _empty_like(x, zero=True) if grad_y is None else _rows(grad_y)
+        W = weight.shape[1]
+        gy = torch.zeros_like(x) if grad_y is None else grad_y
+        gy = gy if gy.stride(-1) == 1 else _rows(gy)
         gl = None if grad_last is None else grad_last.contiguous()
         gx = _empty_like(x)
         make = torch.zeros_like if Bn == 0 or Dn == 0 else torch.empty_like
         gw = make(weight)
         gb, gs = (None if t is None else make(t) for t in (bias, state))
         lib = _capi.lib()
-        args = _conv_args(x, weight, bias, state, lengths, ctx.silu, None, _tb(gy), None)
-        grads = _capi.SHORT_CONV_GRADS.pack(_p(gy), _p(gl), _p(gx), _p(gs), _p(gw), _p(gb), *_tb(gx))
+        args = _conv_args(x, weight, bias, state, lengths, ctx.silu, None, gy.stride()[:2], None)
+        grads = _capi.SHORT_CONV_GRADS.pack(gy.data_ptr(), _p(gl), gx.data_ptr(), _p(gs), gw.data_ptr(),
+                                            _p(gb), *gx.stride()[:2])
         size = lib.dfsnn_short_conv_backward_workspace_size(T, Bn, Dn, W)
-        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        ws = weight.new_empty(size // 4)
         _call(lib.dfsnn_short_conv_backward, "short_conv_backward", 2,
-              lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), True), dev, args, grads,
-              ws.data_ptr(), ws.numel())
+              lambda: _prof.short_conv_bytes(T, Bn, Dn, W, x.element_size(), True), x.get_device(), args,
+              grads, ws.data_ptr(), size)
         return gx, gw, gb, gs, None, None, None
 
 
@@ -389,14 +401,15 @@ def short_conv(x, weight, bias=None, activation=None, state=None, lengths=None, 
     silu = _silu_flag(activation, name)
     x = _lead(x, name, 3)
     T, Bn, Dn = x.shape
+    dev = x.get_device()
     if T < 1:
         raise ValueError(f"{name}: at least one step, got T = {T}")
     W = _taps(weight, Dn, name)
-    weight = _param(weight, x.device, (Dn, W), name, "weight")
-    bias = _param(bias, x.device, (Dn,), name, "bias")
+    weight = _param(weight, dev, (Dn, W), name, "weight")
+    bias = _param(bias, dev, (Dn,), name, "bias")
     if state is not None:
-        state = _seq(state, x, (Bn, W - 1, Dn), name, "state").contiguous()
-    lengths = _integers(lengths, x.device, Bn, name, "lengths")
+        state = _seq(state, x.dtype, dev, (Bn, W - 1, Dn), name, "state").contiguous()
+    lengths = _integers(lengths, dev, Bn, name, "lengths")
     tensors = (x, weight, bias, state)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         y, last = ShortConvFunction.apply(*tensors, lengths, silu, bool(return_state))
@@ -413,17 +426,18 @@ def short_conv_step(x, state, weight, bias=None, activation=None, index=None, st
     name = "short_conv_step"
     silu = _silu_flag(activation, name)
     x = _lead(x, name, 2)
-    Bn, Dn = x.shape
-    W, dev = _taps(weight, Dn, name), x.device
+    shape, dtype, dev = x.shape, x.dtype, x.get_device()
+    Bn, Dn = shape
+    W = _taps(weight, Dn, name)
     weight = _param(weight, dev, (Dn, W), name, "weight")
     bias = _param(bias, dev, (Dn,), name, "bias")
     index = _integers(index, dev, Bn, name, "index")
-    state, state_out, slots = _pool(state, state_out, dev, x.dtype, (W - 1, Dn), Bn, index, name)
-    y = torch.empty((Bn, Dn), dtype=x.dtype, device=dev)
+    state_out, slots, s_in, s_out = _pool(state, state_out, dtype, dev, (W - 1, Dn), Bn, index, name)
+    y = x.new_empty(shape)
     args = _capi.SHORT_CONV_STEP_ARGS.pack(
-        _p(x), _p(weight), _p(bias), _p(state), _p(state_out), _p(index), _p(y), x.stride(0), Dn,
-        state.stride(0), state_out.stride(0), Bn, Dn, slots, W, _DTYPES[x.dtype], silu,
-        int(index is not None and index.dtype == torch.int64))
+        x.data_ptr(), weight.data_ptr(), _p(bias), state.data_ptr(), state_out.data_ptr(), _p(index),
+        y.data_ptr(), x.stride(0), Dn, s_in, s_out, Bn, Dn, slots, W, _DTYPES[dtype], silu,
+        int(index is not None and index.dtype is torch.int64))
     _call(_capi.lib().dfsnn_short_conv_step, name, 1,
           lambda: _prof.short_conv_step_bytes(Bn, Dn, W, x.element_size()), dev, args)
     return y
