@@ -3,59 +3,94 @@
 //   p_t = bias + sum_j w_j x_(t-W+1+j),   y_t = p_t or p_t sigmoid(p_t)
 //
 // Every form reads its sequences once and writes once: bound by memory.  A warp takes 32 * V
-// neighbouring channels (V elements make one 16-byte access where rows are aligned, else V = 1)
-// and a run of steps, along which the last W - 1 inputs stay in registers; W is a template
-// argument, so they do.  Sums are fp32; outputs are rounded once.
+// neighbouring channels (V elements make one 16- or 8-byte access where rows are aligned) and a run
+// of steps, along which the last W - 1 inputs stay in registers; W is a template argument, so they
+// do.  The next 8 to 16 steps are on their way meanwhile, through a ring in shared memory of which
+// each thread copies and reads its own part (no barriers, no registers), and the arithmetic is
+// packed by pairs of channels.  Sums are fp32; outputs are rounded once.
 #include <algorithm>
 
 #include "short_conv.h"
+#include "state_tile.cuh"
 
 namespace dfsnn {
 namespace {
 
 constexpr int NT = 256, NW = NT / 32;
 
+// V neighbouring elements of a row, as they come and as pairs of floats (V = 1: one of the pair)
 template <typename IO, int V>
-struct Row {
-    static __device__ __forceinline__ void load(float (&f)[V], const IO* p) {
-        if constexpr (V == 1) {
-            f[0] = to_f(*p);
-        } else {
-            IO r[V];
-            if constexpr (sizeof(IO) * V == 16) *reinterpret_cast<uint4*>(r) = *reinterpret_cast<const uint4*>(p);
-            else *reinterpret_cast<uint2*>(r) = *reinterpret_cast<const uint2*>(p);
+struct __align__(V * sizeof(IO) > 16 ? 16 : V * sizeof(IO)) Row {
+    IO v[V];
+    static constexpr int P = (V + 1) / 2;
+    __device__ __forceinline__ void get(float2 (&f)[P]) const {
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = to_f(r[i]);
-        }
+        for (int i = 0; i < P; ++i) f[i] = make_float2(to_f(v[2 * i]), V == 1 ? 0.0f : to_f(v[V == 1 ? 0 : 2 * i + 1]));
     }
-    static __device__ __forceinline__ void store(IO* p, const float (&f)[V]) {
-        if constexpr (V == 1) {
-            *p = from_f<IO>(f[0]);
-        } else {
-            IO r[V];
+    __device__ __forceinline__ void set(const float2 (&f)[P]) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) r[i] = from_f<IO>(f[i]);
-            if constexpr (sizeof(IO) * V == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(r);
-            else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(r);
-        }
+        for (int i = 0; i < V; ++i) v[i] = from_f<IO>(i % 2 ? f[i / 2].y : f[i / 2].x);
     }
-    static __device__ __forceinline__ void zero(float (&f)[V]) {
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = 0.0f;
+        for (int i = 0; i < V; ++i) v[i] = from_f<IO>(0.0f);
     }
 };
 
-// Input of ext step t (t < 0: the state in front of the sequence), zero outside [-(W-1), len)
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+
+// Input of step t: of the sequence, of the state in front of it (t < 0), or zero
 template <typename IO, int V, int W>
-__device__ __forceinline__ void load_x(float (&f)[V], const IO* x, long long x_t, const IO* state,
-                                       long long channels, long long t, long long len) {
-    if (t >= 0 && t < len) Row<IO, V>::load(f, x + t * x_t);
-    else if (t < 0 && t >= 1 - W && state) Row<IO, V>::load(f, state + (t + W - 1) * channels);
-    else Row<IO, V>::zero(f);
+__device__ __forceinline__ Row<IO, V> load_x(const IO* x, long long x_t, const IO* state, long long channels,
+                                             long long t, long long len) {
+    Row<IO, V> r;
+    if (t >= 0 && t < len) r = *reinterpret_cast<const Row<IO, V>*>(x + t * x_t);
+    else if (t < 0 && t >= 1 - W && state) r = *reinterpret_cast<const Row<IO, V>*>(state + (t + W - 1) * channels);
+    else r.zero();
+    return r;
+}
+
+// A thread's next rows of one sequence, asynchronously, G rows a group.  A row is fetched into the
+// slot that it is read from; the slots of a group are filled again after its last use.
+constexpr int G = 4;
+template <typename IO, int V>
+struct Ring {
+    using R = Row<IO, V>;
+    static constexpr int kBytes = (int)sizeof(R), kGroups = kBytes > 8 ? 2 : 4;
+    static constexpr size_t kSize = (size_t)kGroups * G * NT * kBytes;       // for the block
+    R* mine;
+    __device__ __forceinline__ Ring(void* smem) : mine(static_cast<R*>(smem) + threadIdx.x) {}
+    __device__ __forceinline__ R* at(int slot, int k) const { return mine + (slot * G + k) * NT; }
+    __device__ __forceinline__ void fetch(int slot, int k, const IO* src, const IO* any, bool ok) const {
+        if constexpr (kBytes >= 4) {
+            copy_async<kBytes>(at(slot, k), ok ? src : any, ok ? kBytes : 0);
+        } else {
+            R r;
+            r.zero();
+            if (ok) r = *reinterpret_cast<const R*>(src);
+            *at(slot, k) = r;
+        }
+    }
+};
+
+// Weights as pairs of channels: w[i][j] for channels 2i, 2i + 1
+template <int V, int W>
+__device__ __forceinline__ void load_weights(float2 (&w)[(V + 1) / 2][W], float2 (&bias)[(V + 1) / 2],
+                                             const dfsnn_short_conv_args& a, long long c) {
+#pragma unroll
+    for (int i = 0; i < (V + 1) / 2; ++i) {
+        const int o = V == 1 ? 0 : 1;
+        bias[i] = a.bias ? make_float2(a.bias[c + 2 * i], a.bias[c + 2 * i + o]) : two(0.0f);
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            w[i][j] = make_float2(a.weight[(c + 2 * i) * W + j], a.weight[(c + 2 * i + o) * W + j]);
+    }
 }
 
 template <typename IO, int V, int W>
-__global__ void __launch_bounds__(NT) conv_fwd(const ConvParams p) {
+__global__ void __launch_bounds__(NT, W <= 4 ? 3 : 1) conv_fwd(const ConvParams p) {
+    constexpr int P = (V + 1) / 2;
+    using R = Row<IO, V>;
     const dfsnn_short_conv_args& a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long item = (long long)(blockIdx.x / p.channel_blocks) * NW + warp;
@@ -66,49 +101,65 @@ __global__ void __launch_bounds__(NT) conv_fwd(const ConvParams p) {
     const IO* x = static_cast<const IO*>(a.x) + b * a.x_b + c;
     const IO* state = a.state ? static_cast<const IO*>(a.state) + b * (W - 1) * a.channels + c : nullptr;
     IO* y = static_cast<IO*>(a.y) + b * a.y_b + c;
-
-    float w[V][W], bias[V], win[W][V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = a.bias ? a.bias[c + i] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = a.weight[(c + i) * W + j];
-    }
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j)
-        load_x<IO, V, W>(win[j + 1], x, a.x_t, state, a.channels, t0 - (W - 1) + j, len);
-
     const long long t1 = t0 + p.run < a.T ? t0 + p.run : a.T;
-    constexpr int U = 4;                        // steps loaded ahead
-    for (long long t = t0; t < t1; t += U) {
-        float in[U][V];
+    const long long lim = t1 < len ? t1 : len;
+
+    extern __shared__ __align__(16) unsigned char smem[];
+    const Ring<IO, V> ring(smem);
+    constexpr int N = Ring<IO, V>::kGroups;
+    const IO* ahead = x + t0 * a.x_t;           // next row to fetch
+    long long t_ahead = t0;
+    auto fetch = [&](int slot) {
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            load_x<IO, V, W>(in[k], x, a.x_t, nullptr, 0, t + k, t1 < len ? t1 : len);
+        for (int k = 0; k < G; ++k) {
+            ring.fetch(slot, k, ahead, x, t_ahead + k < lim);
+            ahead += a.x_t;
+        }
+        t_ahead += G;
+        copy_commit();
+    };
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-            float o[V];
+    for (int n = 0; n < N; ++n) fetch(n);
+    float2 w[P][W], bias[P], win[W][P];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+    for (int j = 1; j < W; ++j) load_x<IO, V, W>(x, a.x_t, state, a.channels, t0 - W + j, len).get(win[j]);
+    load_weights<V, W>(w, bias, a, c);
+    IO* yt = y + t0 * a.y_t;
+    int slot = 0;
+    for (long long t = t0; t < t1; t += G) {
+        copy_wait<N - 1>();
+        const bool inner = t + G <= lim;        // all of them in the run and in the sequence
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+            float2 f[P], o[P];
+            ring.at(slot, k)->get(f);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
 #pragma unroll
                 for (int j = 0; j < W - 1; ++j) win[j][i] = win[j + 1][i];
-                win[W - 1][i] = in[k][i];
-                float s = bias[i];
+                win[W - 1][i] = f[i];
+                float2 s = bias[i];
 #pragma unroll
-                for (int j = 0; j < W; ++j) s = fmaf(w[i][j], win[j][i], s);
-                o[i] = t + k >= len ? 0.0f : (a.silu ? s * sigmoid_f(s) : s);
+                for (int j = 0; j < W; ++j) s = __ffma2_rn(w[i][j], win[j][i], s);
+                o[i] = a.silu ? __fmul2_rn(s, sigmoid_f(s)) : s;
             }
-            if (t + k < t1) Row<IO, V>::store(y + (t + k) * a.y_t, o);
+            if (inner || t + k < t1) {
+                R out;
+                out.set(o);
+                if (!inner && t + k >= len) out.zero();
+                *reinterpret_cast<R*>(yt) = out;
+            }
+            yt += a.y_t;
         }
+        fetch(slot);
+        slot = slot + 1 == N ? 0 : slot + 1;
     }
     if (a.last && t0 == 0) {
         IO* last = static_cast<IO*>(a.last) + b * (W - 1) * a.channels + c;
 #pragma unroll
-        for (int j = 0; j < W - 1; ++j) {
-            float f[V];
-            load_x<IO, V, W>(f, x, a.x_t, state, a.channels, len - (W - 1) + j, len);
-            Row<IO, V>::store(last + j * a.channels, f);
-        }
+        for (int j = 0; j < W - 1; ++j)
+            *reinterpret_cast<R*>(last + j * a.channels) =
+                load_x<IO, V, W>(x, a.x_t, state, a.channels, len - (W - 1) + j, len);
     }
 }
 
@@ -116,25 +167,21 @@ __global__ void __launch_bounds__(NT) conv_fwd(const ConvParams p) {
 // Walking forwards, gp_t completes the gradient of step s = t - (W - 1); a run therefore goes
 // W - 1 steps past its end, and the first run starts at the state (s = -(W - 1)).
 template <typename IO, int V, int W>
-__global__ void __launch_bounds__(NT) conv_bwd(const ConvParams p) {
+__global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams p) {
+    constexpr int P = (V + 1) / 2;
+    using R = Row<IO, V>;
     __shared__ float s_sum[NW][32 * V];
+    extern __shared__ __align__(16) unsigned char smem[];
+    const Ring<IO, V> ring(smem), gring(smem + Ring<IO, V>::kSize);
+    constexpr int N = Ring<IO, V>::kGroups;
     const dfsnn_short_conv_args& a = p.a;
     const dfsnn_short_conv_grads& g = p.g;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int part = blockIdx.x / p.channel_blocks;
     const long long c = ((long long)(blockIdx.x % p.channel_blocks) * 32 + lane) * V;
     const bool c_ok = c < a.channels;
-    float w[V][W], bias[V], gw[V][W], gb[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias[i] = c_ok && a.bias ? a.bias[c + i] : 0.0f;
-        gb[i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            w[i][j] = c_ok ? a.weight[(c + i) * W + j] : 0.0f;
-            gw[i][j] = 0.0f;
-        }
-    }
+    float2 w[P][W] = {}, bias[P] = {}, gw[P][W] = {}, gb[P] = {};
+    if (c_ok) load_weights<V, W>(w, bias, a, c);
     for (long long item = (long long)part * NW + warp; c_ok && item < p.items;
          item += (long long)p.parts * NW) {
         const long long b = item / p.runs, t0 = item % p.runs * p.run;
@@ -144,86 +191,106 @@ __global__ void __launch_bounds__(NT) conv_bwd(const ConvParams p) {
         const IO* state = a.state ? static_cast<const IO*>(a.state) + b * (W - 1) * a.channels + c : nullptr;
         const IO* gy = static_cast<const IO*>(g.grad_y) + b * a.y_b + c;
         const IO* glast = g.grad_last ? static_cast<const IO*>(g.grad_last) + b * (W - 1) * a.channels + c : nullptr;
-        IO* gx = static_cast<IO*>(g.grad_x) + b * g.gx_b + c;
         IO* gstate = g.grad_state ? static_cast<IO*>(g.grad_state) + b * (W - 1) * a.channels + c : nullptr;
-        float win[W][V], gp[W][V];              // x_(t-W+1 .. t), gp_(t-W+1 .. t)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            Row<IO, V>::zero(gp[j]);
-            if (j > 0) load_x<IO, V, W>(win[j], x, a.x_t, state, a.channels, t0 - W + j, len);
-        }
         // Steps of this run: gp from t0; the gradients complete from t0 on (from -(W-1) in the
         // first run), the last W - 1 of them only with the next run's gp.
-        const long long end = t1 + W - 1;
-        constexpr int U = 4;
-        for (long long t = t0; t < end; t += U) {
-            float in[U][V], gin[U][V];
+        const long long end = t1 + W - 1, lim = end < len ? end : len;
+        const IO *ahead = x + t0 * a.x_t, *gahead = gy + t0 * a.y_t;    // next rows to fetch
+        long long t_ahead = t0;
+        auto fetch = [&](int slot) {
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const long long lim = end < len ? end : len;
-                load_x<IO, V, W>(in[k], x, a.x_t, nullptr, 0, t + k, lim);
-                if (t + k < lim) Row<IO, V>::load(gin[k], gy + (t + k) * a.y_t);
-                else Row<IO, V>::zero(gin[k]);
+            for (int k = 0; k < G; ++k) {
+                ring.fetch(slot, k, ahead, x, t_ahead + k < lim);
+                gring.fetch(slot, k, gahead, gy, t_ahead + k < lim);
+                ahead += a.x_t;
+                gahead += a.y_t;
             }
+            t_ahead += G;
+            copy_commit();
+        };
+        copy_wait<0>();                         // what is left of the last run's fetches
 #pragma unroll
-            for (int k = 0; k < U; ++k) {
-                const bool mine = t + k < t1;   // sums of the parameters: each step once
-                float o[V];
+        for (int n = 0; n < N; ++n) fetch(n);
+        float2 win[W][P], gp[W][P] = {};        // x_(t-W+1 .. t), gp_(t-W+1 .. t)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
+        for (int j = 1; j < W; ++j) load_x<IO, V, W>(x, a.x_t, state, a.channels, t0 - W + j, len).get(win[j]);
+        IO* gx = static_cast<IO*>(g.grad_x) + b * g.gx_b + c + (t0 - (W - 1)) * g.gx_t;
+        const long long inner_end = t1 < len ? t1 : len;
+        int slot = 0;
+        for (long long t = t0; t < end; t += G) {
+            copy_wait<N - 1>();
+            // gp and the completed gradients all in the run and in the sequence
+            const bool inner = t >= t0 + W - 1 && t + G <= inner_end;
+#pragma unroll
+            for (int k = 0; k < G; ++k) {
+                float2 f[P], v[P], o[P];
+                ring.at(slot, k)->get(f);
+                gring.at(slot, k)->get(v);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
 #pragma unroll
                     for (int j = 0; j < W - 1; ++j) {
                         win[j][i] = win[j + 1][i];
                         gp[j][i] = gp[j + 1][i];
                     }
-                    win[W - 1][i] = in[k][i];
-                    float v = gin[k][i];
+                    win[W - 1][i] = f[i];
                     if (a.silu) {
-                        float s = bias[i];
+                        float2 s = bias[i];
 #pragma unroll
-                        for (int j = 0; j < W; ++j) s = fmaf(w[i][j], win[j][i], s);
-                        const float sg = sigmoid_f(s);
-                        v *= fmaf(s * sg, 1.0f - sg, sg);
+                        for (int j = 0; j < W; ++j) s = __ffma2_rn(w[i][j], win[j][i], s);
+                        const float2 sg = sigmoid_f(s), si = __fmul2_rn(s, sg);
+                        // silu' = sg + si (1 - sg)
+                        v[i] = __fmul2_rn(v[i], __ffma2_rn(si, __ffma2_rn(sg, two(-1.0f), two(1.0f)), sg));
                     }
-                    if (t + k >= len) v = 0.0f;
-                    gp[W - 1][i] = v;
-                    if (mine) {
-                        gb[i] += v;
+                    if (!inner && t + k >= lim) v[i] = two(0.0f);
+                    gp[W - 1][i] = v[i];
+                    if (inner || t + k < t1) {  // sums of the parameters: each step in one run only
+                        gb[i] = __fadd2_rn(gb[i], v[i]);
 #pragma unroll
-                        for (int j = 0; j < W; ++j) gw[i][j] = fmaf(v, win[j][i], gw[i][j]);
+                        for (int j = 0; j < W; ++j) gw[i][j] = __ffma2_rn(v[i], win[j][i], gw[i][j]);
                     }
-                    float s = 0.0f;
+                    float2 s = __fmul2_rn(w[i][0], gp[W - 1][i]);
 #pragma unroll
-                    for (int j = 0; j < W; ++j) s = fmaf(w[i][j], gp[W - 1 - j][i], s);
+                    for (int j = 1; j < W; ++j) s = __ffma2_rn(w[i][j], gp[W - 1 - j][i], s);
                     o[i] = s;
                 }
-                const long long s = t + k - (W - 1);
-                if (s >= (t0 == 0 ? 1 - W : t0) && s < t1) {
-                    if (glast && s >= len - (W - 1) && s < len) {
-                        float f[V];
-                        Row<IO, V>::load(f, glast + (s - (len - (W - 1))) * a.channels);
+                R out;
+                if (inner) {
+                    out.set(o);
+                    *reinterpret_cast<R*>(gx) = out;
+                } else {
+                    const long long s = t + k - (W - 1);
+                    if (s >= (t0 == 0 ? 1 - W : t0) && s < t1) {
+                        if (glast && s >= len - (W - 1) && s < len) {
+                            float2 l[P];
+                            reinterpret_cast<const R*>(glast + (s - (len - (W - 1))) * a.channels)->get(l);
 #pragma unroll
-                        for (int i = 0; i < V; ++i) o[i] += f[i];
-                    }
-                    if (s >= 0) {
-                        if (s >= len) Row<IO, V>::zero(o);
-                        Row<IO, V>::store(gx + s * g.gx_t, o);
-                    } else if (gstate) {
-                        Row<IO, V>::store(gstate + (s + W - 1) * a.channels, o);
+                            for (int i = 0; i < P; ++i) o[i] = __fadd2_rn(o[i], l[i]);
+                        }
+                        out.set(o);
+                        if (s >= 0) {
+                            if (s >= len) out.zero();
+                            *reinterpret_cast<R*>(gx) = out;
+                        } else if (gstate) {
+                            *reinterpret_cast<R*>(gstate + (s + W - 1) * a.channels) = out;
+                        }
                     }
                 }
+                gx += g.gx_t;
             }
+            fetch(slot);
+            slot = slot + 1 == N ? 0 : slot + 1;
         }
     }
+    copy_wait<0>();
     // over the warps of the block, in order; then one row of parts for the block
+#pragma unroll
     for (int j = 0; j <= W; ++j) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            float v = gb[i];
-#pragma unroll
-            for (int q = 0; q < W; ++q) v = j == q ? gw[i][q] : v;
-            s_sum[warp][lane * V + i] = v;
+            const float2 v = j < W ? gw[i / 2][j < W ? j : 0] : gb[i / 2];
+            s_sum[warp][lane * V + i] = i % 2 ? v.y : v.x;
         }
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * V; i += NT) {
@@ -238,16 +305,26 @@ __global__ void __launch_bounds__(NT) conv_bwd(const ConvParams p) {
     }
 }
 
-// grad weight and grad bias from the blocks' parts: a warp for 32 / 8 outputs ... in a fixed order
-__global__ void conv_bwd_sums(const ConvParams p, int W) {
-    const long long total = p.a.channels * (W + 1);
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= total) return;
-    const long long j = i / p.a.channels, c = i % p.a.channels;
+// grad weight and grad bias from the blocks' parts, 32 outputs a block: its 8 warps add every eighth
+// part, then the warps' sums are added in order
+__global__ void __launch_bounds__(NT) conv_bwd_sums(const ConvParams p, int W) {
+    __shared__ float s_sum[NW][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long total = p.a.channels * (W + 1), i = (long long)blockIdx.x * 32 + lane;
     float v = 0.0f;
-    for (int q = 0; q < p.parts; ++q) v += p.part[q * total + i];
-    if (j < W) p.g.grad_weight[c * W + j] = v;
-    else if (p.g.grad_bias) p.g.grad_bias[c] = v;
+    if (i < total) {
+#pragma unroll 4
+        for (int q = warp; q < p.parts; q += NW) v += p.part[q * total + i];
+    }
+    s_sum[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && i < total) {
+        v = 0.0f;
+        for (int q = 0; q < NW; ++q) v += s_sum[q][lane];
+        const long long j = i / p.a.channels, c = i % p.a.channels;
+        if (j < W) p.g.grad_weight[c * W + j] = v;
+        else if (p.g.grad_bias) p.g.grad_bias[c] = v;
+    }
 }
 
 template <typename IO, int V, int W>
@@ -256,30 +333,43 @@ __global__ void __launch_bounds__(128) conv_step(const dfsnn_short_conv_step_arg
     const long long c = ((long long)(blockIdx.x % tiles) * 128 + threadIdx.x) * V;
     const long long slot = step_slot(a.index, a.index64, b, a.slots);
     if (c >= a.channels) return;
-    IO* y = static_cast<IO*>(a.y) + b * a.y_b + c;
-    float o[V];
+    using R = Row<IO, V>;
+    constexpr int P = R::P;
+    R* y = reinterpret_cast<R*>(static_cast<IO*>(a.y) + b * a.y_b + c);
     if (slot < 0) {
+        float2 o[P];
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = slot == kIdle ? 0.0f : __int_as_float(0x7fc00000);
-        Row<IO, V>::store(y, o);
+        for (int i = 0; i < P; ++i) o[i] = two(slot == kIdle ? 0.0f : __int_as_float(0x7fc00000));
+        y->set(o);
         return;
     }
     const IO* in = static_cast<const IO*>(a.state) + slot * a.state_s + c;
     IO* out = static_cast<IO*>(a.state_out) + slot * a.out_s + c;
-    float win[W][V];
+    R row[W];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) Row<IO, V>::load(win[j], in + j * a.channels);
-    Row<IO, V>::load(win[W - 1], static_cast<const IO*>(a.x) + b * a.x_b + c);
+    for (int j = 0; j < W - 1; ++j) row[j] = *reinterpret_cast<const R*>(in + j * a.channels);
+    row[W - 1] = *reinterpret_cast<const R*>(static_cast<const IO*>(a.x) + b * a.x_b + c);
+    dfsnn_short_conv_args weights{};
+    weights.weight = a.weight;
+    weights.bias = a.bias;
+    float2 w[P][W], s[P];
+    load_weights<V, W>(w, s, weights, c);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float s = a.bias ? a.bias[c + i] : 0.0f;
+    for (int j = 0; j < W; ++j) {
+        float2 f[P];
+        row[j].get(f);
 #pragma unroll
-        for (int j = 0; j < W; ++j) s = fmaf(a.weight[(c + i) * W + j], win[j][i], s);
-        o[i] = a.silu ? s * sigmoid_f(s) : s;
+        for (int i = 0; i < P; ++i) s[i] = __ffma2_rn(w[i][j], f[i], s[i]);
+    }
+    if (a.silu) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) s[i] = __fmul2_rn(s[i], sigmoid_f(s[i]));
     }
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) Row<IO, V>::store(out + j * a.channels, win[j + 1]);
-    Row<IO, V>::store(y, o);
+    for (int j = 0; j < W - 1; ++j) *reinterpret_cast<R*>(out + j * a.channels) = row[j + 1];
+    R o;
+    o.set(s);
+    *y = o;
 }
 
 // Whether rows of this tensor can be read V elements at a time
@@ -305,16 +395,19 @@ cudaError_t launch(Form form, ConvParams& p, const dfsnn_short_conv_step_args* s
     if (form == Form::kForward) {
         const long long blocks = (p.items + NW - 1) / NW * p.channel_blocks;
         if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-        conv_fwd<IO, V, W><<<(unsigned)blocks, NT, 0, st>>>(p);
+        conv_fwd<IO, V, W><<<(unsigned)blocks, NT, Ring<IO, V>::kSize, st>>>(p);
         return cudaGetLastError();
     }
     const long long blocks = (long long)p.parts * p.channel_blocks;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    conv_bwd<IO, V, W><<<(unsigned)blocks, NT, 0, st>>>(p);
-    cudaError_t e = cudaGetLastError();
+    constexpr size_t smem = 2 * Ring<IO, V>::kSize;
+    cudaError_t e = cudaFuncSetAttribute(conv_bwd<IO, V, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    conv_bwd<IO, V, W><<<(unsigned)blocks, NT, smem, st>>>(p);
+    e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     const long long total = p.a.channels * (W + 1);
-    conv_bwd_sums<<<(unsigned)((total + 127) / 128), 128, 0, st>>>(p, W);
+    conv_bwd_sums<<<(unsigned)((total + 31) / 32), NT, 0, st>>>(p, W);
     return cudaGetLastError();
 }
 
@@ -332,25 +425,27 @@ cudaError_t pick_taps(Form form, ConvParams& p, const dfsnn_short_conv_step_args
     }
 }
 
+// Whether every row of a call starts on a multiple of V elements
+template <typename IO, int V>
+bool fits(Form form, const ConvParams& p, const dfsnn_short_conv_step_args* s) {
+    constexpr int E = (int)sizeof(IO);
+    constexpr size_t B = V * sizeof(IO);
+    if (form == Form::kStep)
+        return s->channels % V == 0 && rows_fit(s->x, B, {s->x_b}, E) && rows_fit(s->y, B, {s->y_b}, E)
+               && rows_fit(s->state, B, {s->state_s}, E) && rows_fit(s->state_out, B, {s->out_s}, E);
+    if (p.a.channels % V || !rows_fit(p.a.x, B, {p.a.x_t, p.a.x_b}, E) || !rows_fit(p.a.state, B, {}, E)) return false;
+    if (form == Form::kForward)
+        return rows_fit(p.a.y, B, {p.a.y_t, p.a.y_b}, E) && rows_fit(p.a.last, B, {}, E);
+    return rows_fit(p.g.grad_y, B, {p.a.y_t, p.a.y_b}, E) && rows_fit(p.g.grad_x, B, {p.g.gx_t, p.g.gx_b}, E)
+           && rows_fit(p.g.grad_last, B, {}, E) && rows_fit(p.g.grad_state, B, {}, E);
+}
+
+// 8-byte accesses (16 for fp32) where rows allow it, else pairs of channels, else single ones.
 template <typename IO>
 cudaError_t pick(Form form, ConvParams& p, const dfsnn_short_conv_step_args* s, cudaStream_t st) {
-    constexpr int V = 4, E = (int)sizeof(IO);
-    const size_t B = V * sizeof(IO);
-    bool fit;
-    if (form == Form::kStep) {
-        fit = s->channels % V == 0 && rows_fit(s->x, B, {s->x_b}, E) && rows_fit(s->y, B, {s->y_b}, E)
-              && rows_fit(s->state, B, {s->state_s}, E) && rows_fit(s->state_out, B, {s->out_s}, E);
-    } else {
-        fit = p.a.channels % V == 0 && rows_fit(p.a.x, B, {p.a.x_t, p.a.x_b}, E)
-              && rows_fit(p.a.state, B, {}, E);
-        if (form == Form::kForward)
-            fit = fit && rows_fit(p.a.y, B, {p.a.y_t, p.a.y_b}, E) && rows_fit(p.a.last, B, {}, E);
-        else
-            fit = fit && rows_fit(p.g.grad_y, B, {p.a.y_t, p.a.y_b}, E)
-                  && rows_fit(p.g.grad_x, B, {p.g.gx_t, p.g.gx_b}, E)
-                  && rows_fit(p.g.grad_last, B, {}, E) && rows_fit(p.g.grad_state, B, {}, E);
-    }
-    return fit ? pick_taps<IO, V>(form, p, s, st) : pick_taps<IO, 1>(form, p, s, st);
+    if (fits<IO, 4>(form, p, s)) return pick_taps<IO, 4>(form, p, s, st);
+    if (fits<IO, 2>(form, p, s)) return pick_taps<IO, 2>(form, p, s, st);
+    return pick_taps<IO, 1>(form, p, s, st);
 }
 
 cudaError_t run(Form form, int dtype, ConvParams& p, const dfsnn_short_conv_step_args* s, cudaStream_t st) {
@@ -361,9 +456,12 @@ cudaError_t run(Form form, int dtype, ConvParams& p, const dfsnn_short_conv_step
     }
 }
 
-// Runs of up to 32 steps: the W - 1 rows that a run reads twice stay few
+// Runs of 64 steps, or fewer (down to 8) where that would leave warps without work: the W - 1 rows
+// that a run reads twice stay few.
 void set_runs(ConvParams& p) {
-    p.run = 32;
+    const long long lanes = (p.a.channels + 127) / 128;
+    p.run = 64;
+    while (p.run > 8 && (p.a.T + p.run - 1) / p.run * p.a.batch * lanes < 148 * 32) p.run /= 2;
     p.runs = (p.a.T + p.run - 1) / p.run;
     p.items = p.runs * p.a.batch;
 }
@@ -382,6 +480,7 @@ int short_conv_parts(long long T, long long batch, long long channels) {
     ConvParams p{};
     p.a.T = T;
     p.a.batch = batch;
+    p.a.channels = channels;
     set_runs(p);
     const long long blocks = (p.items + NW - 1) / NW, cb = (channels + 127) / 128;
     return (int)std::max<long long>(1, std::min(blocks, (148 * 8 + cb - 1) / cb));
