@@ -73,17 +73,30 @@ struct Ring {
     }
 };
 
-// Weights as pairs of channels: w[i][j] for channels 2i, 2i + 1
+// Weights as pairs of channels: w[i][j] for channels 2i, 2i + 1.  Those of V = 4 channels are W
+// 16-byte accesses (fits() has seen to it).
 template <int V, int W>
 __device__ __forceinline__ void load_weights(float2 (&w)[(V + 1) / 2][W], float2 (&bias)[(V + 1) / 2],
-                                             const dfsnn_short_conv_args& a, long long c) {
+                                             const float* weight, const float* b, long long c) {
+    float f[V * W], g[V];
+    if constexpr (V == 4) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+            *reinterpret_cast<float4*>(f + 4 * i) = __ldg(reinterpret_cast<const float4*>(weight + c * W) + i);
+        const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<float4*>(g) = b ? __ldg(reinterpret_cast<const float4*>(b + c)) : none;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V * W; ++i) f[i] = weight[c * W + i];
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[i] = b ? b[c + i] : 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < (V + 1) / 2; ++i) {
-        const int o = V == 1 ? 0 : 1;
-        bias[i] = a.bias ? make_float2(a.bias[c + 2 * i], a.bias[c + 2 * i + o]) : two(0.0f);
+        const int o = V == 1 ? 0 : 2 * i + 1;
+        bias[i] = make_float2(g[2 * i], g[o]);
 #pragma unroll
-        for (int j = 0; j < W; ++j)
-            w[i][j] = make_float2(a.weight[(c + 2 * i) * W + j], a.weight[(c + 2 * i + o) * W + j]);
+        for (int j = 0; j < W; ++j) w[i][j] = make_float2(f[2 * i * W + j], f[o * W + j]);
     }
 }
 
@@ -123,7 +136,7 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 3 : 1) conv_fwd(const ConvParams 
     float2 w[P][W], bias[P], win[W][P];
 #pragma unroll
     for (int j = 1; j < W; ++j) load_x<IO, V, W>(x, a.x_t, state, a.channels, t0 - W + j, len).get(win[j]);
-    load_weights<V, W>(w, bias, a, c);
+    load_weights<V, W>(w, bias, a.weight, a.bias, c);
     IO* yt = y + t0 * a.y_t;
     int slot = 0;
     for (long long t = t0; t < t1; t += G) {
@@ -181,7 +194,7 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams 
     const long long c = ((long long)(blockIdx.x % p.channel_blocks) * 32 + lane) * V;
     const bool c_ok = c < a.channels;
     float2 w[P][W] = {}, bias[P] = {}, gw[P][W] = {}, gb[P] = {};
-    if (c_ok) load_weights<V, W>(w, bias, a, c);
+    if (c_ok) load_weights<V, W>(w, bias, a.weight, a.bias, c);
     for (long long item = (long long)part * NW + warp; c_ok && item < p.items;
          item += (long long)p.parts * NW) {
         const long long b = item / p.runs, t0 = item % p.runs * p.run;
@@ -331,11 +344,21 @@ template <typename IO, int V, int W>
 __global__ void __launch_bounds__(128) conv_step(const dfsnn_short_conv_step_args a, int tiles) {
     const long long b = blockIdx.x / tiles;
     const long long c = ((long long)(blockIdx.x % tiles) * 128 + threadIdx.x) * V;
-    const long long slot = step_slot(a.index, a.index64, b, a.slots);
-    if (c >= a.channels) return;
     using R = Row<IO, V>;
     constexpr int P = R::P;
+    long long slot = step_slot(a.index, a.index64, b, a.slots);
+    const bool ours = slot >= 0, c_ok = c < a.channels;
+    const IO* in = static_cast<const IO*>(a.state) + slot * a.state_s + c;      // not read unless the slot is one
+    IO* out = static_cast<IO*>(a.state_out) + slot * a.out_s + c;
     R* y = reinterpret_cast<R*>(static_cast<IO*>(a.y) + b * a.y_b + c);
+    R row[W];
+    if (ours && c_ok) {
+#pragma unroll
+        for (int j = 0; j < W - 1; ++j) row[j] = *reinterpret_cast<const R*>(in + j * a.channels);
+        row[W - 1] = *reinterpret_cast<const R*>(static_cast<const IO*>(a.x) + b * a.x_b + c);
+    }
+    if (taken_before(a.index, a.index64, b, slot) && ours) slot = kBad;
+    if (!c_ok) return;
     if (slot < 0) {
         float2 o[P];
 #pragma unroll
@@ -343,17 +366,8 @@ __global__ void __launch_bounds__(128) conv_step(const dfsnn_short_conv_step_arg
         y->set(o);
         return;
     }
-    const IO* in = static_cast<const IO*>(a.state) + slot * a.state_s + c;
-    IO* out = static_cast<IO*>(a.state_out) + slot * a.out_s + c;
-    R row[W];
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) row[j] = *reinterpret_cast<const R*>(in + j * a.channels);
-    row[W - 1] = *reinterpret_cast<const R*>(static_cast<const IO*>(a.x) + b * a.x_b + c);
-    dfsnn_short_conv_args weights{};
-    weights.weight = a.weight;
-    weights.bias = a.bias;
     float2 w[P][W], s[P];
-    load_weights<V, W>(w, s, weights, c);
+    load_weights<V, W>(w, s, a.weight, a.bias, c);
 #pragma unroll
     for (int j = 0; j < W; ++j) {
         float2 f[P];
@@ -430,6 +444,8 @@ template <typename IO, int V>
 bool fits(Form form, const ConvParams& p, const dfsnn_short_conv_step_args* s) {
     constexpr int E = (int)sizeof(IO);
     constexpr size_t B = V * sizeof(IO);
+    const float *weight = form == Form::kStep ? s->weight : p.a.weight, *bias = form == Form::kStep ? s->bias : p.a.bias;
+    if (V == 4 && ((reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(bias)) & 15)) return false;
     if (form == Form::kStep)
         return s->channels % V == 0 && rows_fit(s->x, B, {s->x_b}, E) && rows_fit(s->y, B, {s->y_b}, E)
                && rows_fit(s->state, B, {s->state_s}, E) && rows_fit(s->state_out, B, {s->out_s}, E);

@@ -115,25 +115,25 @@ struct LaneSums {
     }
 };
 
-// Slot of row b of a step call.  kIdle: a negative index; kBad: behind the last slot, or the slot
-// of an earlier row (two rows of one call cannot both advance it).  All threads of the block
-// call it together.
+// Slot of row b of a step call: its index; kIdle for a negative one, kBad behind the last slot.
+// taken_before: whether an earlier row has the same slot (two rows of one call cannot both advance
+// it, so the later one is refused).  It is found out while the state is on its way: reading a slot
+// harms nobody.  All threads of the block call it together.
 constexpr long long kIdle = -1, kBad = -2;
 __device__ __forceinline__ long long index_at(const void* index, int wide, long long b) {
     return wide ? static_cast<const long long*>(index)[b]
                 : (long long)static_cast<const int*>(index)[b];
 }
-__device__ __forceinline__ long long step_slot(const void* index, int wide, long long b,
-                                               long long slots) {
+__device__ __forceinline__ long long step_slot(const void* index, int wide, long long b, long long slots) {
     if (index == nullptr) return b;
     const long long slot = index_at(index, wide, b);
+    return slot < 0 ? kIdle : slot >= slots ? kBad : slot;
+}
+__device__ __forceinline__ bool taken_before(const void* index, int wide, long long b, long long slot) {
+    if (index == nullptr) return false;
     bool taken = false;
-    if (slot >= 0)
-        for (long long r = threadIdx.x; r < b; r += blockDim.x)
-            taken |= index_at(index, wide, r) == slot;
-    taken = __syncthreads_or(taken);
-    if (slot < 0) return kIdle;
-    return taken || slot >= slots ? kBad : slot;
+    for (long long r = threadIdx.x; r < b; r += blockDim.x) taken |= index_at(index, wide, r) == slot;
+    return __syncthreads_or(taken);
 }
 
 }  // namespace dfsnn

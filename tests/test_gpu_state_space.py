@@ -235,7 +235,9 @@ def step_case(B, D, N, G, dtype, slots, seed=0):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (1, 130, 16, 1), (3, 96, 12, 3), (5, 33, 4, 1), (2, 40, 8, 2),
                                      (2, 20, 5, 1), (4, 24, 32, 2), (2, 10, 17, 1), (3, 12, 64, 1), (2, 9, 100, 3),
-                                     (2, 7, 128, 1), (2, 6, 127, 2)])
+                                     (2, 7, 128, 1), (2, 6, 127, 2),
+                                     (130, 650, 16, 1), (300, 514, 4, 2), (200, 516, 8, 3), (150, 202, 64, 1),
+                                     (100, 330, 32, 2), (160, 515, 12, 1), (90, 701, 3, 1)])
 def test_scan_step_against_64_bits(B, D, N, G, dtype):
     x, row, pool = step_case(B, D, N, G, dtype, B, seed=B + N)
     kw = dict(softplus=True)
