@@ -66,7 +66,7 @@ struct __align__(sizeof(IO) * V) Pack {
 };
 
 template <typename IO, int S, int SL, int C, bool WIDE, bool ENDS>
-__global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
+__global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
     using Tl = Tile<IO, S, SL, C>;
     constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS;
     constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
@@ -251,23 +251,44 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
             }
         }
         constexpr int R = 8;                    // steps whose sums over the lanes are formed together
+        constexpr int G = 4;                    // steps whose operands are read one group ahead
+        static_assert(R == kScanChunk, "states are kept in front of every R steps");
+        float2 d_n[G][C], B_n[G][S / 2], C_n[G][S / 2];
+        auto read = [&](int t0g) {
+#pragma unroll
+            for (int t = 0; t < G; ++t) {
+                load_states<S>(B_n[t], &sh.B[t0g + t][n0]);
+                if (!ENDS) load_states<S>(C_n[t], &sh.C_[t0g + t][n0]);
+#pragma unroll
+                for (int c = 0; c < C; ++c) d_n[t][c] = sh.d[cl + c * CL][t0g + t];
+            }
+        };
+        read(0);
 #pragma unroll
         for (int tr = 0; tr < TT; tr += R) {
-            static_assert(R == kScanChunk, "states are kept in front of every R steps");
             if (!ENDS && a.kept && t0 + tr > 0 && t0 + tr < len)
                 put(a.kept + (long long)((t0 + tr) / R - 1) * a.batch * a.channels * a.states + row);
             float y[C][R];
-            constexpr int G = 4;                // steps whose decays are formed before their states
 #pragma unroll
             for (int tg = 0; tg < R; tg += G) {
-                float2 dec[G][C][S / 2], in[G][C][S / 2];
+                float2 d_c[G][C], B_c[G][S / 2], C_c[G][S / 2];
 #pragma unroll
                 for (int t = 0; t < G; ++t) {
-                    float2 Bv[S / 2];
-                    load_states<S>(Bv, &sh.B[tr + tg + t][n0]);
+#pragma unroll
+                    for (int c = 0; c < C; ++c) d_c[t][c] = d_n[t][c];
+#pragma unroll
+                    for (int j = 0; j < S / 2; ++j) {
+                        B_c[t][j] = B_n[t][j];
+                        if (!ENDS) C_c[t][j] = C_n[t][j];
+                    }
+                }
+                if (tr + tg + G < TT) read(tr + tg + G);
+                float2 dec[G][C][S / 2], in[G][C][S / 2];
+#pragma unroll
+                for (int t = 0; t < G; ++t)
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
-                        const float2 d = sh.d[cl + c * CL][tr + tg + t];
+                        const float2 d = d_c[t][c];
                         const float2 dt = make_float2(d.x, d.x), du = make_float2(d.y, d.y);
                         if (ENDS) steps[c] += d.x;
 #pragma unroll
@@ -275,25 +296,21 @@ __global__ void __launch_bounds__(NT) scan_fwd(const ScanParams p) {
                             const float2 x = __fmul2_rn(dt, A2[c][j]), q = exp2_near1(x);
                             dec[t][c][j] = make_float2(near1[c][2 * j] ? q.x : exp2_approx(x.x),
                                                        near1[c][2 * j + 1] ? q.y : exp2_approx(x.y));
-                            in[t][c][j] = __fmul2_rn(du, Bv[j]);
+                            in[t][c][j] = __fmul2_rn(du, B_c[t][j]);
                         }
                     }
-                }
 #pragma unroll
-                for (int t = 0; t < G; ++t) {
-                    float2 Cv[S / 2];
-                    if (!ENDS) load_states<S>(Cv, &sh.C_[tr + tg + t][n0]);
+                for (int t = 0; t < G; ++t)
 #pragma unroll
                     for (int c = 0; c < C; ++c) {
                         float2 acc;
 #pragma unroll
                         for (int j = 0; j < S / 2; ++j) {
                             h[c][j] = __ffma2_rn(dec[t][c][j], h[c][j], in[t][c][j]);
-                            if (!ENDS) acc = j == 0 ? __fmul2_rn(h[c][j], Cv[j]) : __ffma2_rn(h[c][j], Cv[j], acc);
+                            if (!ENDS) acc = j == 0 ? __fmul2_rn(h[c][j], C_c[t][j]) : __ffma2_rn(h[c][j], C_c[t][j], acc);
                         }
                         if (!ENDS) y[c][tg + t] = acc.x + acc.y;
                     }
-                }
             }
             if (!ENDS) {
                 using Sums = LaneSums<R, SL, CL>;
