@@ -409,13 +409,14 @@ cudaError_t launch(Form form, ConvParams& p, const dfsnn_short_conv_step_args* s
     if (form == Form::kForward) {
         const long long blocks = (p.items + NW - 1) / NW * p.channel_blocks;
         if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+        static_assert(Ring<IO, V>::kSize <= 48 * 1024, "within the default");
         conv_fwd<IO, V, W><<<(unsigned)blocks, NT, Ring<IO, V>::kSize, st>>>(p);
         return cudaGetLastError();
     }
     const long long blocks = (long long)p.parts * p.channel_blocks;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     constexpr size_t smem = 2 * Ring<IO, V>::kSize;
-    cudaError_t e = cudaFuncSetAttribute(conv_bwd<IO, V, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_shared<conv_bwd<IO, V, W>>(smem);
     if (e != cudaSuccess) return e;
     conv_bwd<IO, V, W><<<(unsigned)blocks, NT, smem, st>>>(p);
     e = cudaGetLastError();

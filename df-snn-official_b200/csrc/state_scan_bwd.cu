@@ -14,6 +14,7 @@
 // on over the warps in shared memory and over the blocks through partial sums that a second kernel
 // adds in a fixed order: no atomics, so results do not change from run to run.
 #include <algorithm>
+#include <type_traits>
 
 #include "state_scan.h"
 #include "state_tile.cuh"
@@ -191,12 +192,12 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
         auto fill = [&](int t0) {
             const int rows = len - t0;
             Raw& r = sh.raw[t0 / TT & 1];
-            fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words);
-            fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
-            fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], g_p, a.y_t, rows, cols, p.words);
-            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words);
-            fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
-            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], g_p, a.y_t, rows, cols, p.words, threadIdx.x);
+            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words, threadIdx.x);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words, threadIdx.x);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words, threadIdx.x);
             u_p -= TT * a.u_t;
             d_p -= TT * a.delta_t;
             z_p -= TT * a.z_t;
@@ -264,6 +265,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
             copy_wait<0>();
             __syncthreads();
             if (t0 > first) fill(t0 - TT);
+            const bool tail = t0 + TT > len;
             float2 x_r[E], dt_r[E];                             // the softplus's argument and result
             if (t_e < TT) {
 #pragma unroll
@@ -274,7 +276,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                     float2 dt = __fadd2_rn(unpack<IO, V>(&raw.d[t][ch]), bias);
                     x_r[e] = dt;
                     if (a.softplus) dt = softplus_f(dt);
-                    if (t0 + t >= len) dt = two(0.0f);          // a step behind the end leaves the state alone
+                    if (tail && t0 + t >= len) dt = two(0.0f);  // a step behind the end leaves the state alone
                     dt_r[e] = dt;
                     if (a.z) {
                         const float2 z = unpack<IO, V>(&raw.z[t][ch]);
@@ -423,10 +425,11 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
 
             // elementwise gradients
             if (ch_ok) {
+                IO *gu_t = gu_p + t0 * g.gu_t, *gd_t = gd_p + t0 * g.gdelta_t, *gz_t = gz_p + t0 * g.gz_t;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const int t = t_e + e * TS;
-                    if (t0 + t < stop) {
+                    if (!tail || t0 + t < stop) {
                         const float2 u = unpack<IO, V>(&raw.u[t][ch]);
                         float2 go = unpack<IO, V>(&raw.g[t][ch]), gz = two(0.0f);
                         const float2 lb = make_float2(sh.lb[ch][t], sh.lb[ch + V - 1][t]);
@@ -443,12 +446,12 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                         float2 gd = __ffma2_rn(u, lb, __fmul2_rn(qa, two(0.69314718055994530942f)));
                         if (a.softplus) gd = __fmul2_rn(gd, sigmoid_f(x_r[e]));
                         float2 gu = __ffma2_rn(dt_r[e], lb, __fmul2_rn(skip, go));
-                        if (t0 + t >= len) gd = gu = gz = go = two(0.0f);
-                        store<IO, V>(gu_p + (t0 + e * TS) * g.gu_t, gu);
-                        store<IO, V>(gd_p + (t0 + e * TS) * g.gdelta_t, gd);
-                        if (g.grad_z) store<IO, V>(gz_p + (t0 + e * TS) * g.gz_t, gz);
+                        if (tail && t0 + t >= len) gd = gu = gz = go = two(0.0f);
+                        store<IO, V>(gu_t + e * (TS * g.gu_t), gu);
+                        store<IO, V>(gd_t + e * (TS * g.gdelta_t), gd);
+                        if (g.grad_z) store<IO, V>(gz_t + e * (TS * g.gz_t), gz);
                         sum_bias = __fadd2_rn(sum_bias, gd);
-                        if (t0 + t < len) sum_D = __ffma2_rn(go, u, sum_D);
+                        sum_D = __ffma2_rn(go, tail && t0 + t >= len ? two(0.0f) : u, sum_D);
                     }
                 }
             }
@@ -559,11 +562,11 @@ __global__ void __launch_bounds__(NT) scan_bwd_ends(const ScanParams p) {
         const int rows = len - t0;
         const long long c = g_base + c_base;
         typename Tl::Raw& r = sh.raw[t0 / TT & 1];
-        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], static_cast<const IO*>(a.delta) + b * a.delta_b + c + t0 * a.delta_t, a.delta_t, rows, cols, p.words);
-        fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], static_cast<const IO*>(p.g.grad_y) + b * a.y_b + c + t0 * a.y_t, a.y_t, rows, cols, p.words);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], static_cast<const IO*>(a.delta) + b * a.delta_b + c + t0 * a.delta_t, a.delta_t, rows, cols, p.words, threadIdx.x);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], static_cast<const IO*>(p.g.grad_y) + b * a.y_b + c + t0 * a.y_t, a.y_t, rows, cols, p.words, threadIdx.x);
         if (a.z)
-            fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], static_cast<const IO*>(a.z) + b * a.z_b + c + t0 * a.z_t, a.z_t, rows, cols, p.words);
-        fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + t0 * a.C_t, a.C_t, rows, a.states, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], static_cast<const IO*>(a.z) + b * a.z_b + c + t0 * a.z_t, a.z_t, rows, cols, p.words, threadIdx.x);
+        fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + t0 * a.C_t, a.C_t, rows, a.states, p.words, threadIdx.x);
         copy_commit();
     };
     const int top = (len - 1) / TT * TT;
@@ -632,18 +635,36 @@ __global__ void __launch_bounds__(kSumThreads) scan_bwd_sums(const ScanParams p,
     const long long n_bc = (long long)p.T * a.batch * a.groups * a.states;
     const long long n_a = a.channels * a.states;
     if (blockIdx.x < bc_blocks) {
-        for (long long i = (long long)blockIdx.x * kSumThreads + threadIdx.x; i < 2 * n_bc;
-             i += (long long)bc_blocks * kSumThreads) {
-            float v = 0.0f;
-            const int which = i >= n_bc;
-            const long long k = i - which * n_bc, row = k / (a.groups * a.states);
-            if (row / a.batch < seq_length(a.lengths, a.lengths64, row % a.batch, p.T)) {
-                const float* q = p.part_bc + (long long)which * p.tiles * n_bc + k;
-#pragma unroll 4
-                for (int j = 0; j < p.tiles; ++j) v += q[j * n_bc];
+        // W neighbouring states of a (step, sequence, group) at a time
+        auto add = [&](auto width) {
+            constexpr int W = decltype(width)::value;
+            for (long long i = (long long)blockIdx.x * kSumThreads + threadIdx.x; i < 2 * n_bc / W;
+                 i += (long long)bc_blocks * kSumThreads) {
+                const int which = i >= n_bc / W;
+                const long long k = (i - which * (n_bc / W)) * W, row = k / (a.groups * a.states);
+                float v[W] = {};
+                if (row / a.batch < seq_length(a.lengths, a.lengths64, row % a.batch, p.T)) {
+                    const float* q = p.part_bc + (long long)which * p.tiles * n_bc + k;
+#pragma unroll 8
+                    for (int j = 0; j < p.tiles; ++j, q += n_bc) {
+                        if constexpr (W == 4) {
+                            const float4 f = __ldcs(reinterpret_cast<const float4*>(q));
+                            v[0] += f.x;
+                            v[1] += f.y;
+                            v[2] += f.z;
+                            v[3] += f.w;
+                        } else {
+                            v[0] += *q;
+                        }
+                    }
+                }
+                IO* out = static_cast<IO*>(which ? g.grad_C : g.grad_B) + k;
+#pragma unroll
+                for (int w = 0; w < W; ++w) out[w] = from_f<IO>(v[w]);
             }
-            static_cast<IO*>(which ? g.grad_C : g.grad_B)[k] = from_f<IO>(v);
-        }
+        };
+        if (a.states % 4 == 0) add(std::integral_constant<int, 4>{});      // rows of parts lie on 16 bytes
+        else add(std::integral_constant<int, 1>{});
         return;
     }
     __shared__ float s_sum[kSumThreads / 32][32];
@@ -691,14 +712,12 @@ cudaError_t launch_form(const ScanParams& p, cudaStream_t st) {
         q.tiles = (p.group_channels + Ends::BC - 1) / Ends::BC;
         const long long n = (long long)q.tiles * p.a.groups * p.a.batch * (p.splits - 1);
         if (n > 0x7fffffffLL) return cudaErrorInvalidValue;
-        cudaError_t e = cudaFuncSetAttribute(scan_bwd_ends<IO, S, SL, WIDE>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Ends));
+        cudaError_t e = allow_shared<scan_bwd_ends<IO, S, SL, WIDE>>(sizeof(Ends));
         if (e != cudaSuccess) return e;
         scan_bwd_ends<IO, S, SL, WIDE><<<(unsigned)n, NT, sizeof(Ends), st>>>(q);
     }
     constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
-    cudaError_t e = cudaFuncSetAttribute(scan_bwd<IO, S, SL, C, WIDE>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = allow_shared<scan_bwd<IO, S, SL, C, WIDE>>(smem);
     if (e != cudaSuccess) return e;
     scan_bwd<IO, S, SL, C, WIDE><<<(unsigned)blocks, NT, smem, st>>>(p);
     return cudaGetLastError();

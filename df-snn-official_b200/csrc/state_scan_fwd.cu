@@ -132,12 +132,12 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
             pieces.template issue<Tl::kEights, 1>(stage * (unsigned)sizeof(Raw), rows);
         } else {
             Raw& r = sh.raw[stage];
-            fill_tile<IO, TT, BC, NT, false>(r.u[0], u_p, a.u_t, rows, cols, p.words);
-            fill_tile<IO, TT, BC, NT, false>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
-            fill_tile<IO, TT, NS, NT, false>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+            fill_tile<IO, TT, BC, NT, false>(r.u[0], u_p, a.u_t, rows, cols, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, false>(r.d[0], d_p, a.delta_t, rows, cols, p.words, threadIdx.x);
+            fill_tile<IO, TT, NS, NT, false>(r.B[0], B_p, a.B_t, rows, a.states, p.words, threadIdx.x);
             if (!ENDS) {
-                if (a.z) fill_tile<IO, TT, BC, NT, false>(r.z[0], z_p, a.z_t, rows, cols, p.words);
-                fill_tile<IO, TT, NS, NT, false>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
+                if (a.z) fill_tile<IO, TT, BC, NT, false>(r.z[0], z_p, a.z_t, rows, cols, p.words, threadIdx.x);
+                fill_tile<IO, TT, NS, NT, false>(r.C_[0], C_p, a.C_t, rows, a.states, p.words, threadIdx.x);
             }
             u_p += TT * a.u_t;
             d_p += TT * a.delta_t;
@@ -370,14 +370,9 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
 template <typename IO, int S, int SL, int C, bool WIDE>
 cudaError_t launch_form(const ScanParams& p, unsigned blocks, cudaStream_t st) {
     constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(scan_fwd<IO, S, SL, C, WIDE, true>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(scan_fwd<IO, S, SL, C, WIDE, false>,
-                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
+    cudaError_t e = allow_shared<scan_fwd<IO, S, SL, C, WIDE, false>>(smem);
+    if (e == cudaSuccess && p.splits > 1) e = allow_shared<scan_fwd<IO, S, SL, C, WIDE, true>>(smem);
+    if (e != cudaSuccess) return e;
     if (p.splits > 1)
         scan_fwd<IO, S, SL, C, WIDE, true><<<blocks * (p.splits - 1), NT, smem, st>>>(p);
     scan_fwd<IO, S, SL, C, WIDE, false><<<blocks * p.splits, NT, smem, st>>>(p);

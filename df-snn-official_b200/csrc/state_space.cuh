@@ -1,6 +1,7 @@
 // state_space.cuh -- shared device helpers of the state-space kernels (selective scan, short
 // causal convolution, and their single-token forms).
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -134,6 +135,22 @@ __device__ __forceinline__ bool taken_before(const void* index, int wide, long l
     bool taken = false;
     for (long long r = threadIdx.x; r < b; r += blockDim.x) taken |= index_at(index, wide, r) == slot;
     return __syncthreads_or(taken);
+}
+
+// Lets Kernel use `bytes` of dynamic shared memory on the current device: the driver is asked once
+// for each device.
+template <auto Kernel>
+inline cudaError_t allow_shared(size_t bytes) {
+    static std::atomic<unsigned long long> done{0};
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 }  // namespace dfsnn
