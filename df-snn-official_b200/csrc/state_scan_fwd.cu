@@ -42,7 +42,12 @@ struct Tile {
     template <int COLS> static constexpr int kPieces = Pieces<1>::template kPieces<COLS>;
     static constexpr bool kEights = BC * sizeof(IO) < 16 || NS * sizeof(IO) < 16;   // rows of 8 bytes
     __align__(16) Raw raw[2];                          // this tile's and the next one's
-    float2 d[BC][TT + 1];                              // (d, d u)
+    // (d, d u) of a channel, even channels in front of odd ones: a warp then writes the pairs of a
+    // step, and reads its channels, without bank conflicts
+    float2 d_[BC * (TT + 1) + 4];
+    __device__ __forceinline__ float2* d(int ch) {
+        return d_ + (ch >> 1) * (TT + 1) + (ch & 1) * (BC / 2 * (TT + 1) + 4);
+    }
     __align__(16) float B[TT][NS], C_[TT][NS];
     float o[BC][TT + 1];
 };
@@ -66,7 +71,7 @@ struct __align__(sizeof(IO) * V) Pack {
 };
 
 template <typename IO, int S, int SL, int C, bool WIDE, bool ENDS>
-__global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
+__global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     using Tl = Tile<IO, S, SL, C>;
     constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS;
     constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
@@ -206,12 +211,15 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
         get(a.h0 ? a.h0 + row : nullptr, h);                    // an empty sequence keeps its state
     }
     float steps[C] = {};                                        // sums of d
+    const long long all_states = a.batch * a.channels * a.states;
+    float* kept = a.kept + row - all_states;                    // of step t at t / R * all_states
 
     for (int t0 = first; t0 < len; t0 += TT) {
         const Raw& raw = sh.raw[(t0 - first) / TT & 1];
         copy_wait<0>();
         __syncthreads();
         if (t0 + TT < len) fill(t0 + TT);
+        const bool tail = t0 + TT > len;
         if (t_e < TT) {
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -220,11 +228,11 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
                 const Elem d = *reinterpret_cast<const Elem*>(&raw.d[t][ch]);
                 float2 dt = make_float2(to_f(d.v[0]) + bias[0], to_f(d.v[V - 1]) + bias[V - 1]);
                 if (a.softplus) dt = softplus_f(dt);
-                if (t0 + t >= len) dt = make_float2(0.0f, 0.0f);    // a step behind the end leaves the state alone
+                if (tail && t0 + t >= len) dt = make_float2(0.0f, 0.0f);   // a step behind the end leaves the state alone
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const float x = v ? dt.y : dt.x;
-                    sh.d[ch + v][t] = make_float2(x, x * to_f(u.v[v]));
+                    sh.d(ch + v)[t] = make_float2(x, x * to_f(u.v[v]));
                 }
             }
         }
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
             float most = 0.0f;
 #pragma unroll
             for (int t = 0; t < TT; t += SL)
-                if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d[cl + c * CL][t + (SL <= TT ? sl : sl % TT)].x));
+                if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d(cl + c * CL)[t + (SL <= TT ? sl : sl % TT)].x));
 #pragma unroll
             for (int m = SL / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m * CL));
 #pragma unroll
@@ -251,7 +259,7 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
             }
         }
         constexpr int R = 8;                    // steps whose sums over the lanes are formed together
-        constexpr int G = 4;                    // steps whose operands are read one group ahead
+        constexpr int G = 2;                    // steps whose operands are read one group ahead
         static_assert(R == kScanChunk, "states are kept in front of every R steps");
         float2 d_n[G][C], B_n[G][S / 2], C_n[G][S / 2];
         auto read = [&](int t0g) {
@@ -260,14 +268,14 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
                 load_states<S>(B_n[t], &sh.B[t0g + t][n0]);
                 if (!ENDS) load_states<S>(C_n[t], &sh.C_[t0g + t][n0]);
 #pragma unroll
-                for (int c = 0; c < C; ++c) d_n[t][c] = sh.d[cl + c * CL][t0g + t];
+                for (int c = 0; c < C; ++c) d_n[t][c] = sh.d(cl + c * CL)[t0g + t];
             }
         };
         read(0);
 #pragma unroll
         for (int tr = 0; tr < TT; tr += R) {
             if (!ENDS && a.kept && t0 + tr > 0 && t0 + tr < len)
-                put(a.kept + (long long)((t0 + tr) / R - 1) * a.batch * a.channels * a.states + row);
+                put(kept + (long long)((t0 + tr) / R) * all_states);
             float y[C][R];
 #pragma unroll
             for (int tg = 0; tg < R; tg += G) {
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int t = t_e + e * TS;
-            if (ch_ok && t0 + t < stop) {
+            if (ch_ok && (!tail || t0 + t < stop)) {
                 const Elem u = *reinterpret_cast<const Elem*>(&raw.u[t][ch]);
                 const Elem z = *reinterpret_cast<const Elem*>(&raw.z[t][ch]);
                 float2 o = make_float2(fmaf(skip[0], to_f(u.v[0]), sh.o[ch][t]),
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(NT, 4) scan_fwd(const ScanParams p) {
                     const float2 zf = make_float2(to_f(z.v[0]), to_f(z.v[V - 1]));
                     o = __fmul2_rn(o, __fmul2_rn(zf, sigmoid_f(zf)));
                 }
-                if (t0 + t >= len) o = make_float2(0.0f, 0.0f);
+                if (tail && t0 + t >= len) o = make_float2(0.0f, 0.0f);
                 Elem out;
                 out.v[0] = from_f<IO>(o.x);
                 out.v[V - 1] = from_f<IO>(V == 1 ? o.x : o.y);
