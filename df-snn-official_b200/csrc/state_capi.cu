@@ -122,6 +122,20 @@ size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, lo
     return backward_plan(p).bytes();
 }
 
+int dfsnn_state_scan_backward_launches(long long T, long long batch, long long channels, int states,
+                                       int groups) {
+    if (check_scan_sizes(T, batch, channels, states, groups) || batch == 0 || channels == 0) return 0;
+    dfsnn_state_scan_args a{};
+    a.T = T;
+    a.batch = batch;
+    a.channels = channels;
+    a.states = states;
+    a.groups = groups;
+    dfsnn::ScanParams p = scan_params(a);
+    backward_plan(p);
+    return p.splits > 1 && !p.chained ? 3 : 2;
+}
+
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g,
                               void* workspace, size_t workspace_bytes, void* stream) {
     if (int s = check_scan(a)) return s;

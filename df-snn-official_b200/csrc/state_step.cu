@@ -115,7 +115,8 @@ __global__ void __launch_bounds__(NT, M == 4 ? 6 : 1) scan_step(const dfsnn_stat
     }
 }
 
-// One channel a thread for few rows (latency); up to four where that still leaves 4 blocks an SM
+// One channel a thread for few rows (latency); up to four where that still leaves 4 blocks an SM:
+// N = 16, bf16, 64 x 2048 5.7 us with four against 8.2 with one, 192 x 4096 25.5 against 49.3
 template <typename IO, int V, int LG, int K>
 cudaError_t launch(const dfsnn_state_scan_step_args& a, cudaStream_t st) {
     constexpr int M = K > 1 ? 1 : LG < 4 ? LG : 4;

@@ -93,6 +93,7 @@ SIGNATURES = {
     "dfsnn_state_scan_forward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
     "dfsnn_state_scan_forward": (_i, [_args, _p, _sz, _p]),
     "dfsnn_state_scan_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
+    "dfsnn_state_scan_backward_launches": (_i, [_ll, _ll, _ll, _i, _i]),
     "dfsnn_state_scan_backward": (_i, [_args, _args, _p, _sz, _p]),
     "dfsnn_state_scan_step": (_i, [_args, _p]),
     "dfsnn_short_conv_forward": (_i, [_args, _p]),

@@ -258,7 +258,8 @@ class StateScanFunction(torch.autograd.Function):
             gA.data_ptr(), _p(gD), _p(gbias), _p(gh0), *gu.stride()[:2], *gdelta.stride()[:2], *_tb(gz))
         size = lib.dfsnn_state_scan_backward_workspace_size(T, Bn, Dn, N, G)
         ws = A.new_empty(size // 4)
-        _call(lib.dfsnn_state_scan_backward, "state_scan_backward", 2,
+        _call(lib.dfsnn_state_scan_backward, "state_scan_backward",
+              2 if _prof._ACTIVE is None else lib.dfsnn_state_scan_backward_launches(T, Bn, Dn, N, G),
               lambda: _prof.state_scan_bytes(T, Bn, Dn, N, G, u.element_size(), z is not None, True),
               u.get_device(), args, grads, ws.data_ptr(), size)
         return gu, gdelta, gA, gB, gC, gD, gz, gbias, gh0, None, None, None

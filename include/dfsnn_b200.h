@@ -424,7 +424,8 @@ typedef struct {
     long long gu_t, gu_b, gdelta_t, gdelta_b, gz_t, gz_b;
 } dfsnn_state_scan_grads;
 
-/* Floats of the `kept` array (the states at every DFSNN_SCAN_CHUNK steps; 0: none needed). */
+/* Floats of the `kept` array (the states in front of every DFSNN_SCAN_CHUNK steps but the first; 0:
+ * none needed). */
 size_t dfsnn_state_scan_kept_floats(long long T, long long batch, long long channels, int states);
 /* Few long sequences are scanned in parts; their states need a workspace (0 bytes otherwise). */
 size_t dfsnn_state_scan_forward_workspace_size(long long T, long long batch, long long channels,
@@ -433,6 +434,9 @@ int dfsnn_state_scan_forward(const dfsnn_state_scan_args* args, void* workspace,
                              size_t workspace_bytes, void* stream);
 size_t dfsnn_state_scan_backward_workspace_size(long long T, long long batch, long long channels,
                                                 int states, int groups);
+/* Kernels that dfsnn_state_scan_backward launches for these sizes (for launch counts). */
+int dfsnn_state_scan_backward_launches(long long T, long long batch, long long channels, int states,
+                                       int groups);
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* args, const dfsnn_state_scan_grads* grads,
                               void* workspace, size_t workspace_bytes, void* stream);
 

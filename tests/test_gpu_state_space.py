@@ -120,12 +120,12 @@ def test_scan_batch_first_views():
 
 @pytest.mark.parametrize("T,B,D,N,G,lengths", [
     (300, 480, 8, 16, 1, None), (270, 64, 250, 12, 2, "ragged"), (290, 300, 33, 4, 1, "ragged")])
-def test_scan_backward_in_rounds(T, B, D, N, G, lengths):
+def test_scan_backward_in_waves(T, B, D, N, G, lengths):
     """More blocks than run at a time: the parts of a sequence run one after another."""
     if lengths:
         lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(T)).tolist()
     x, n, grads = scan_case(T, B, D, N, G, "f32", lengths=lengths, seed=T, scale=0.1)
-    check_scan(x, n, grads, True, f"rounds {T}x{B}x{D}")
+    check_scan(x, n, grads, True, f"waves {T}x{B}x{D}")
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -208,6 +208,52 @@ def test_scan_in_parts_equals_whole():
                            return_state=True)
     # cut at a tile's end: the same operations in the same order
     assert torch.equal(torch.cat([y1, y2]), y) and torch.equal(h2, h)
+
+
+def test_offsets_past_32_bits():
+    """Sequences of more than 2^31 elements: their last rows as in a call of their own."""
+    T, B, D, N, last = 1100, 1030, 2048, 4, 160
+    g = torch.Generator(device=DEV).manual_seed(1)
+    u = torch.randn(T, B, D, generator=g, device=DEV, dtype=torch.bfloat16)
+    dt = torch.rand(T, B, D, generator=g, device=DEV, dtype=torch.bfloat16) * 0.1
+    A, bc = -torch.rand(D, N, device=DEV), torch.randn(T, B, 2, N, generator=g, device=DEV).bfloat16()
+    assert u.numel() > 2 ** 31
+    full, part = ((u, dt, bc), tuple(t[:, -last:].contiguous() for t in (u, dt, bc)))
+
+    def run(u, dt, bc):
+        u, dt = u.detach().requires_grad_(True), dt.detach().requires_grad_(True)
+        y = ss.state_scan(u, dt, A, bc[:, :, :1], bc[:, :, 1:])
+        return [y.detach()[:, -last:], *(v[:, -last:] for v in torch.autograd.grad(y, (u, dt), torch.ones_like(y)))]
+    for a, b in zip(run(*full), run(*part)):
+        assert torch.equal(a, b)
+    w = torch.randn(D, 4, device=DEV)
+
+    def conv(u):
+        u = u.detach().requires_grad_(True)
+        y = ss.short_conv(u, w, None, "silu")
+        return [y.detach()[:, -last:], torch.autograd.grad(y, u, torch.ones_like(y))[0][:, -last:]]
+    for a, b in zip(conv(u), conv(part[0])):
+        assert torch.equal(a, b)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with parts that wait for one another or side by side."""
+    cases = [scan_case(T, B, D, 16, 1, "f32", seed=40 + T) for T, B, D in ((300, 480, 8), (260, 500, 30), (900, 1, 64))]
+    leaves = [{k: v.requires_grad_(True) for k, v in x.items()} for x, _, _ in cases]
+
+    def run(i):
+        y, h = ss.state_scan(**leaves[i], softplus=True, return_state=True)
+        return [y, h, *torch.autograd.grad([y, h], list(leaves[i].values()), list(cases[i][2]))]
+    want = [run(i) for i in range(3)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], [None] * 3
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = run(i)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
 def test_empty_batch_and_channels():
@@ -413,12 +459,13 @@ def test_other_stream():
 
 
 def test_graph_replay():
-    """Two captured training passes and a captured step, replayed in turn on new inputs.  (An eager
-    graph of the same leaves must not live while a backward is captured: torch's own gradient
-    nodes of the leaves would wait for the stream of that graph, and the capture fails.)"""
+    """Captured training passes (whole sequences, parts side by side, parts one after another) and a
+    captured step, replayed in turn on new inputs.  (An eager graph of the same leaves must not live
+    while a backward is captured: torch's own gradient nodes of the leaves would wait for the stream
+    of that graph, and the capture fails.)"""
     graphs = []
-    for seed, (T, D) in enumerate(((40, 96), (17, 64))):
-        x, _, (gy, _) = scan_case(T, 2, D, 16, 1, "bf16", seed=20 + seed)
+    for seed, (T, B, D, launches) in enumerate(((40, 2, 96, 6), (17, 2, 64, 6), (700, 1, 64, 8), (300, 480, 8, 6))):
+        x, _, (gy, _) = scan_case(T, B, D, 16, 1, "bf16", seed=20 + seed)
         leaves = {k: v.requires_grad_(True) for k, v in x.items()}
         w = torch.randn(D, 4, device=DEV, requires_grad=True)
 
@@ -434,7 +481,7 @@ def test_graph_replay():
         g = torch.cuda.CUDAGraph()
         with profiling.NativeCallTimer() as timer, torch.cuda.graph(g):
             out = run()
-        assert timer.captured_launches() == 6
+        assert timer.captured_launches() == launches
         graphs.append((g, out, run, leaves))
     x, row, pool = step_case(4, 64, 16, 1, "bf16", 4, seed=30)
     new, index = torch.empty_like(pool), torch.tensor([3, -1, 0, 2], dtype=torch.int32, device=DEV)
