@@ -61,9 +61,9 @@ struct Ring {
     R* mine;
     __device__ __forceinline__ Ring(void* smem) : mine(static_cast<R*>(smem) + threadIdx.x) {}
     __device__ __forceinline__ R* at(int slot, int k) const { return mine + (slot * G + k) * NT; }
-    __device__ __forceinline__ void fetch(int slot, int k, const IO* src, const IO* any, bool ok) const {
+    __device__ __forceinline__ void fetch(int slot, int k, const IO* src, bool ok) const {
         if constexpr (kBytes >= 4) {
-            copy_async<kBytes>(at(slot, k), ok ? src : any, ok ? kBytes : 0);
+            copy_async<kBytes>(at(slot, k), src, ok ? kBytes : 0);     // 0: nothing is read
         } else {
             R r;
             r.zero();
@@ -109,23 +109,24 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 3 : 1) conv_fwd(const ConvParams 
     const long long item = (long long)(blockIdx.x / p.channel_blocks) * NW + warp;
     const long long c = ((long long)(blockIdx.x % p.channel_blocks) * 32 + lane) * V;
     if (item >= p.items || c >= a.channels) return;
-    const long long b = item / p.runs, t0 = item % p.runs * p.run;
-    const long long len = seq_length(a.lengths, a.lengths64, b, (int)a.T);
+    const long long b = item / p.runs;
+    const int t0 = (int)(item % p.runs * p.run), T = (int)a.T;     // steps fit 32 bits, offsets do not
+    const int len = seq_length(a.lengths, a.lengths64, b, T);
     const IO* x = static_cast<const IO*>(a.x) + b * a.x_b + c;
     const IO* state = a.state ? static_cast<const IO*>(a.state) + b * (W - 1) * a.channels + c : nullptr;
     IO* y = static_cast<IO*>(a.y) + b * a.y_b + c;
-    const long long t1 = t0 + p.run < a.T ? t0 + p.run : a.T;
-    const long long lim = t1 < len ? t1 : len;
+    const int run = (int)p.run, t1 = T - t0 > run ? t0 + run : T;
+    const int lim = t1 < len ? t1 : len;
 
     extern __shared__ __align__(16) unsigned char smem[];
     const Ring<IO, V> ring(smem);
     constexpr int N = Ring<IO, V>::kGroups;
     const IO* ahead = x + t0 * a.x_t;           // next row to fetch
-    long long t_ahead = t0;
+    int t_ahead = t0;
     auto fetch = [&](int slot) {
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-            ring.fetch(slot, k, ahead, x, t_ahead + k < lim);
+            ring.fetch(slot, k, ahead, t_ahead + k < lim);
             ahead += a.x_t;
         }
         t_ahead += G;
@@ -139,7 +140,7 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 3 : 1) conv_fwd(const ConvParams 
     load_weights<V, W>(w, bias, a.weight, a.bias, c);
     IO* yt = y + t0 * a.y_t;
     int slot = 0;
-    for (long long t = t0; t < t1; t += G) {
+    for (int t = t0; t < t1; t += G) {
         copy_wait<N - 1>();
         const bool inner = t + G <= lim;        // all of them in the run and in the sequence
 #pragma unroll
@@ -197,9 +198,10 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams 
     if (c_ok) load_weights<V, W>(w, bias, a.weight, a.bias, c);
     for (long long item = (long long)part * NW + warp; c_ok && item < p.items;
          item += (long long)p.parts * NW) {
-        const long long b = item / p.runs, t0 = item % p.runs * p.run;
-        const long long t1 = t0 + p.run < a.T ? t0 + p.run : a.T;
-        const long long len = seq_length(a.lengths, a.lengths64, b, (int)a.T);
+        const long long b = item / p.runs;
+        const int t0 = (int)(item % p.runs * p.run), T = (int)a.T, run = (int)p.run;
+        const int t1 = T - t0 > run ? t0 + run : T;
+        const int len = seq_length(a.lengths, a.lengths64, b, T);
         const IO* x = static_cast<const IO*>(a.x) + b * a.x_b + c;
         const IO* state = a.state ? static_cast<const IO*>(a.state) + b * (W - 1) * a.channels + c : nullptr;
         const IO* gy = static_cast<const IO*>(g.grad_y) + b * a.y_b + c;
@@ -207,14 +209,14 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams 
         IO* gstate = g.grad_state ? static_cast<IO*>(g.grad_state) + b * (W - 1) * a.channels + c : nullptr;
         // Steps of this run: gp from t0; the gradients complete from t0 on (from -(W-1) in the
         // first run), the last W - 1 of them only with the next run's gp.
-        const long long end = t1 + W - 1, lim = end < len ? end : len;
+        const int end = t1 + W - 1, lim = end < len ? end : len;
         const IO *ahead = x + t0 * a.x_t, *gahead = gy + t0 * a.y_t;    // next rows to fetch
-        long long t_ahead = t0;
+        int t_ahead = t0;
         auto fetch = [&](int slot) {
 #pragma unroll
             for (int k = 0; k < G; ++k) {
-                ring.fetch(slot, k, ahead, x, t_ahead + k < lim);
-                gring.fetch(slot, k, gahead, gy, t_ahead + k < lim);
+                ring.fetch(slot, k, ahead, t_ahead + k < lim);
+                gring.fetch(slot, k, gahead, t_ahead + k < lim);
                 ahead += a.x_t;
                 gahead += a.y_t;
             }
@@ -228,9 +230,9 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams 
 #pragma unroll
         for (int j = 1; j < W; ++j) load_x<IO, V, W>(x, a.x_t, state, a.channels, t0 - W + j, len).get(win[j]);
         IO* gx = static_cast<IO*>(g.grad_x) + b * g.gx_b + c + (t0 - (W - 1)) * g.gx_t;
-        const long long inner_end = t1 < len ? t1 : len;
+        const int inner_end = t1 < len ? t1 : len;
         int slot = 0;
-        for (long long t = t0; t < end; t += G) {
+        for (int t = t0; t < end; t += G) {
             copy_wait<N - 1>();
             // gp and the completed gradients all in the run and in the sequence
             const bool inner = t >= t0 + W - 1 && t + G <= inner_end;
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(NT, W <= 4 ? 2 : 1) conv_bwd(const ConvParams 
                     out.set(o);
                     *reinterpret_cast<R*>(gx) = out;
                 } else {
-                    const long long s = t + k - (W - 1);
+                    const int s = t + k - (W - 1);
                     if (s >= (t0 == 0 ? 1 - W : t0) && s < t1) {
                         if (glast && s >= len - (W - 1) && s < len) {
                             float2 l[P];
