@@ -13,6 +13,7 @@ struct ScanParams {
     int T, group_channels;
     int tiles;                                 // channel tiles of a group
     bool words;                                // rows_aligned(4), for rows that are not on 16 bytes
+    long long seq_blocks;                      // forward: blocks that share the batch
     // a sequence in parts (splits > 1): `split_steps` steps each, a multiple of the chunk
     int splits, split_steps;
     float* ends;                               // [splits][batch][channels][states] (forward: all but

@@ -91,12 +91,10 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     bid /= a.groups;
     const int parts = ENDS ? p.splits - 1 : p.splits;
     const int split = (int)(bid % parts);
-    const long long b = bid / parts;
-    const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T);
+    const long long b0 = bid / parts;                           // sequences b0, b0 + seq_blocks, ...
     const int first = split * p.split_steps;                    // this part's steps: first .. len - 1,
     const int stop = p.T - first < p.split_steps ? p.T : first + p.split_steps;   // its rows: .. stop - 1
-    const int len = whole_len < stop ? whole_len : stop;
-    if (ENDS && whole_len <= stop) return;                      // no part behind this one
+    if (ENDS && seq_length(a.lengths, a.lengths64, b0, p.T) <= stop) return;      // no part behind this one
     const int c_base = tile * BC;                               // within the group
     const long long g_base = (long long)grp * p.group_channels; // first channel of the group
 
@@ -110,29 +108,15 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
         bias[v] = ch_ok && a.delta_bias ? a.delta_bias[chan + v] : 0.0f;
         skip[v] = !ENDS && ch_ok && a.D ? a.D[chan + v] : 0.0f;
     }
-    IO* y_p = static_cast<IO*>(a.y) + b * a.y_b + chan + (first + t_e) * a.y_t;
-    // the block's sequences at step `first`
-    const IO* u_p = static_cast<const IO*>(a.u) + b * a.u_b + g_base + c_base + first * a.u_t;
-    const IO* d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + g_base + c_base + first * a.delta_t;
-    const IO* z_p = static_cast<const IO*>(a.z) + b * a.z_b + g_base + c_base + first * a.z_t;
-    const IO* B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + first * a.B_t;
-    const IO* C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + first * a.C_t;
     const int cols = p.group_channels - c_base;
     using Raw = typename Tl::Raw;
-    Raw& raw0 = sh.raw[0];
     constexpr int K = ((ENDS ? 2 : 3) * Tl::template kPieces<BC> + (ENDS ? 1 : 2) * Tl::template kPieces<NS> + NT - 1) / NT;
     typename Tl::template Pieces<WIDE ? K : 1> pieces;
-    if constexpr (WIDE) {
-        pieces.template add<BC>(raw0.u, u_p, a.u_t, cols);
-        pieces.template add<BC>(raw0.d, d_p, a.delta_t, cols);
-        pieces.template add<NS>(raw0.B, B_p, a.B_t, a.states);
-        if (!ENDS) {
-            pieces.template add<NS>(raw0.C_, C_p, a.C_t, a.states);
-            if (a.z) pieces.template add<BC>(raw0.z, z_p, a.z_t, cols);
-        }
-    }
+    // the sequence that is being fetched, at the next step to fetch; tiles fetched and scanned so far
+    const IO *u_p = nullptr, *d_p = nullptr, *z_p = nullptr, *B_p = nullptr, *C_p = nullptr;
+    int len_ahead = 0, fetched = 0, scanned = 0;
     auto fill = [&](int t0) {
-        const int stage = (t0 - first) / TT & 1, rows = len - t0;
+        const int stage = fetched++ & 1, rows = len_ahead - t0;
         if constexpr (WIDE) {
             pieces.template issue<Tl::kEights, 1>(stage * (unsigned)sizeof(Raw), rows);
         } else {
@@ -152,11 +136,31 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
         }
         copy_commit();
     };
-    if (first < len) fill(first);                               // in flight while the states are set up
+    auto open = [&](long long b) {
+        const int n = seq_length(a.lengths, a.lengths64, b, p.T);
+        len_ahead = n < stop ? n : stop;
+        u_p = static_cast<const IO*>(a.u) + b * a.u_b + g_base + c_base + first * a.u_t;
+        d_p = static_cast<const IO*>(a.delta) + b * a.delta_b + g_base + c_base + first * a.delta_t;
+        z_p = static_cast<const IO*>(a.z) + b * a.z_b + g_base + c_base + first * a.z_t;
+        B_p = static_cast<const IO*>(a.B) + b * a.B_b + grp * a.B_g + first * a.B_t;
+        C_p = static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + first * a.C_t;
+        if constexpr (WIDE) {
+            Raw& r = sh.raw[0];
+            pieces.clear();
+            pieces.template add<BC>(r.u, u_p, a.u_t, cols);
+            pieces.template add<BC>(r.d, d_p, a.delta_t, cols);
+            pieces.template add<NS>(r.B, B_p, a.B_t, a.states);
+            if (!ENDS) {
+                pieces.template add<NS>(r.C_, C_p, a.C_t, a.states);
+                if (a.z) pieces.template add<BC>(r.z, z_p, a.z_t, cols);
+            }
+        }
+        if (first < len_ahead) fill(first);
+    };
+    open(b0);                                                   // in flight while the states are set up
 
     // recurrence role: states n0 .. n0 + S - 1 of channels cl + c * CL of the block
     const int sl = lane / CL, cl = warp * CW + lane % CL, n0 = sl * S;
-    const long long row = ((long long)b * a.channels + g_base + c_base + cl) * a.states + n0;
     const long long crow = (long long)CL * a.states;            // from one channel of a lane to the next
     // a lane's states are one 16-byte access everywhere
     const bool whole = S == 4 && a.states % 4 == 0
@@ -191,6 +195,12 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int j = 0; j < S / 2; ++j) A2[c][j] = make_float2(A2[c][j].x * kLog2e, A2[c][j].y * kLog2e);
+
+    for (long long b = b0; b < a.batch; b += p.seq_blocks) {
+    const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T), len = whole_len < stop ? whole_len : stop;
+    const long long row = (b * a.channels + g_base + c_base + cl) * a.states + n0;
+    const bool another = b + p.seq_blocks < a.batch;            // its first tile is fetched during our last
+    IO* y_p = static_cast<IO*>(a.y) + b * a.y_b + chan + (first + t_e) * a.y_t;
     if constexpr (ENDS) {
     } else if (first < whole_len) {
         get(a.h0 ? a.h0 + row : nullptr, h);
@@ -215,10 +225,11 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     float* kept = a.kept + row - all_states;                    // of step t at t / R * all_states
 
     for (int t0 = first; t0 < len; t0 += TT) {
-        const Raw& raw = sh.raw[(t0 - first) / TT & 1];
+        const Raw& raw = sh.raw[scanned++ & 1];
         copy_wait<0>();
         __syncthreads();
         if (t0 + TT < len) fill(t0 + TT);
+        else if (another) open(b + p.seq_blocks);
         const bool tail = t0 + TT > len;
         if (t_e < TT) {
 #pragma unroll
@@ -355,6 +366,7 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
             y_p += TS * a.y_t;
         }
     }
+    if (first >= len && another) open(b + p.seq_blocks);
     if (ENDS) {
         put(p.ends + split * a.batch * a.channels * a.states + row);
 #pragma unroll
@@ -373,6 +385,7 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
             *reinterpret_cast<Elem*>(y_p) = none;
     }
     if (a.h_last && (first < whole_len ? whole_len <= stop : split == 0 && whole_len == 0)) put(a.h_last + row);
+    }
 }
 
 template <typename IO, int S, int SL, int C, bool WIDE>
@@ -391,7 +404,13 @@ template <typename IO, int S, int SL, int C>
 cudaError_t launch(ScanParams p, cudaStream_t st) {
     constexpr int BC = Tile<IO, S, SL, C>::BC;
     p.tiles = (p.group_channels + BC - 1) / BC;
-    const long long blocks = (long long)p.tiles * p.a.groups * p.a.batch;
+    // Short sequences: one wave of blocks (five an SM) takes them all, several a block, so that the
+    // set-up is paid once and the next sequence is fetched meanwhile (16 steps, 4096 sequences, 256
+    // channels, fp32: 173 us against 205 with a block for each).
+    const long long per = (long long)p.tiles * p.a.groups, slots = 148 * 5;
+    p.seq_blocks = p.a.batch;
+    if (p.T <= 4 * TT && per * p.a.batch >= 4 * slots && per <= slots) p.seq_blocks = slots / per;
+    const long long blocks = per * p.seq_blocks;
     if (blocks > 0x7fffffffLL / p.splits) return cudaErrorInvalidValue;
     const dfsnn_state_scan_args& a = p.a;
     p.words = rows_aligned(p, sizeof(IO), 4);

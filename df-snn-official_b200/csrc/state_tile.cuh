@@ -57,9 +57,10 @@ struct TilePieces {
     long long step[K];                  // bytes from tile to tile
     unsigned dst[K];                    // byte in the stage
     int t[K], n[K];                     // step in the tile, bytes (0: no such piece)
-    int next = 0;                       // pieces dealt so far
+    int next;                           // pieces dealt so far
 
-    __device__ __forceinline__ TilePieces() {
+    __device__ __forceinline__ void clear() {
+        next = 0;
 #pragma unroll
         for (int k = 0; k < K; ++k) n[k] = -1;
     }

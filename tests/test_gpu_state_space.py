@@ -157,6 +157,17 @@ def test_scan_large_batch_shares_blocks():
     check_scan(x, n, grads, True, "large batch")
 
 
+@pytest.mark.parametrize("T,B,D,N,G", [(20, 3100, 5, 16, 1), (50, 1600, 42, 8, 2), (16, 3000, 36, 3, 1)])
+def test_scan_short_sequences_share_blocks(T, B, D, N, G):
+    """Many short sequences: the forward's blocks take several, empty ones among them."""
+    lengths = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(T))
+    lengths[::7] = 0
+    x, n, grads = scan_case(T, B, D, N, G, "f32", lengths=lengths.tolist(), seed=T)
+    check_scan(x, n, grads, True, "short sequences")
+    x, n, grads = scan_case(T, B, D, N, G, "bf16", full=False, state=False, seed=T)
+    check_scan(x, n, grads, False, "short sequences")
+
+
 def test_scan_strong_decay():
     """d A far below zero: the decay underflows to zero."""
     x, n, grads = scan_case(20, 2, 33, 16, 1, "f32", seed=7, scale=300.0)
