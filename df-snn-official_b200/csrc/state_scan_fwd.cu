@@ -441,14 +441,14 @@ int block_channels(int states) {
 
 }  // namespace
 
-// Parts of a sequence.  Blocks that walk whole sequences fill the machine (148 SMs) from about one
-// an SM on; below that the parts pay for the second walk: 4096 steps, bf16, N = 16, 512 channels 49
-// us in parts against 319 us whole, 2048 channels 156 against 322, 4096 channels (128 blocks) 273
-// against 323.  Parts are 4 tiles at least.
+// Parts of a sequence.  Five blocks run on an SM at a time; while a whole walk of each sequence
+// would leave room for three times the blocks, parts pay for their second walk: 4096 steps, bf16,
+// N = 16, microseconds in parts and whole: 512 channels 51 and 319, 2048 channels 135 and 322, 5888
+// channels (184 blocks) 322 and 426.  Parts are 4 tiles at least.
 int state_scan_splits(long long T, long long batch, long long group_channels, int groups, int states) {
     const int bc = block_channels(states);
     const long long blocks = (group_channels + bc - 1) / bc * groups * batch;
-    long long splits = 148 * 3 / (blocks > 0 ? blocks : 1);
+    long long splits = 148 * 5 / (blocks > 0 ? blocks : 1);
     if (splits < 3) return 1;
     splits = std::min(splits, T / (4 * TT));
     return (int)std::max<long long>(1, splits);
