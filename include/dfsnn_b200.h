@@ -441,8 +441,9 @@ int dfsnn_state_scan_backward(const dfsnn_state_scan_args* args, const dfsnn_sta
                               void* workspace, size_t workspace_bytes, void* stream);
 
 /* One step for each of `batch` rows.  Row b reads the state at slot index[b] of `state` and
- * writes the new one to the same slot of `state_out` (which may be `state`); without an index
- * slot b is row b's.  A slot holds [channels, states] floats, slot s at s * state_s (out_s).
+ * writes the new one to the same slot of `state_out` (`state` itself, or memory that does not
+ * overlap it); without an index slot b is row b's.  A slot holds [channels, states] floats, slot s
+ * at s * state_s (out_s).
  * index[b] < 0: an idle row, whose y is 0.  index[b] >= slots, or the slot of an earlier row:
  * y is NaN and no state is touched.  Sequence tensors have element (b, c) at b * x_b + c. */
 typedef struct {
