@@ -577,3 +577,33 @@ def test_layer_into_neuron():
             assert rel(layer(x[t]), y64[t].detach()) < 2000 * 2.0 ** -24
         layer.reset()
         assert rel(layer(x[0]), y64[0].detach()) < 2000 * 2.0 ** -24
+
+
+def test_layer_serves_from_a_pool():
+    """Padded prompts, their states into a pool, then tokens of some of them with an idle row in
+    between: each sequence as if it were alone, and the pool's other slots untouched."""
+    torch.manual_seed(1)
+    layer = ss.StateSpaceLayer(40, d_state=12, taps=3, groups=4).to(DEV)
+    T, lengths, slots = 12, [9, 3, 6], [5, 0, 2]
+    x = torch.randn(T, 3, 40, device=DEV)
+    n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    rel = lambda a, b: float((a.double() - b.double()).norm() / b.double().norm())  # noqa: E731
+    with torch.no_grad():
+        alone = [layer(x[:, b:b + 1])[:, 0] for b in range(3)]
+        y, (conv, scan) = layer(x, lengths=n, return_state=True)
+        for b, k in enumerate(lengths):                 # the same sums in another grid: fp32 roundings
+            assert rel(y[:k, b], alone[b][:k]) < 2000 * 2.0 ** -24
+        pool = layer.initial_state(7)
+        for p, s in zip(pool, (conv, scan)):
+            p[:] = float("nan")
+            p[slots] = s
+        at = list(lengths)
+        for order in ([2, None, 0, 1], [None, 1, 2], [0]):
+            rows = torch.stack([torch.full((40,), float("nan"), device=DEV) if b is None else x[at[b], b] for b in order])
+            index = torch.tensor([-1 if b is None else slots[b] for b in order], device=DEV)
+            out = layer.step(rows, pool, index)
+            for r, b in enumerate(order):
+                if b is not None:
+                    assert rel(out[r], alone[b][at[b]]) < 2000 * 2.0 ** -24
+                    at[b] += 1
+        assert all(torch.isnan(p[[1, 3, 4, 6]]).all() for p in pool)
