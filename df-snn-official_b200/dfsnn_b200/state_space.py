@@ -151,7 +151,9 @@ def _pool(state, state_out, dtype, dev, inner, rows, index, name):
             raise ValueError(f"{name}: state_out must have {slots} slots, got {out_slots}")
     if index is None and slots < rows:
         raise ValueError(f"{name}: {rows} rows need as many slots, got {slots}")
-    if torch.is_grad_enabled() and not state_out.is_inference():
+    # as torch's in-place operations do, with or without gradients: a sequence call that saved these
+    # states (h0, the convolution's inputs) then refuses its backward
+    if not state_out.is_inference():
         torch.autograd.graph.increment_version(state_out)
     return state_out, slots, stride, out_stride
 

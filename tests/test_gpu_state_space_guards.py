@@ -1,0 +1,56 @@
+"""State-space layer on the GPU: calls that must not return a wrong answer silently."""
+import pytest
+import torch
+
+from dfsnn_b200 import state_space as ss
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def rand(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+# ---------------------------------------------------------------------------------------
+# states written in place
+# ---------------------------------------------------------------------------------------
+def test_scan_state_advanced_before_the_backward_is_noticed():
+    """h0 is saved by reference: a step that advances it must make the backward refuse."""
+    T, B, D, N = 8, 2, 12, 4
+    A, h0 = (-rand(D, N).abs()).requires_grad_(True), rand(B, D, N, seed=1)
+    u, bc = rand(T, B, D, seed=2), rand(T, B, N, seed=3)
+    for step in (torch.no_grad, torch.inference_mode):
+        y = ss.state_scan(u, u, A, bc, bc, softplus=True, h0=h0)
+        with step():
+            ss.state_scan_step(u[0], u[0], h0, A, bc[0], bc[0], softplus=True)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), A)
+
+
+def test_conv_state_advanced_before_the_backward_is_noticed():
+    x, w, state = rand(8, 2, 12), rand(12, 4, seed=1).requires_grad_(True), rand(2, 3, 12, seed=2)
+    y = ss.short_conv(x, w, state=state)
+    with torch.no_grad():
+        ss.short_conv_step(x[0], state, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), w)
+
+
+def test_layer_step_on_a_saved_state_is_noticed():
+    """The prompt's states advanced by a token between its forward and its backward; on copies of
+    them the gradients are those without the token."""
+    torch.manual_seed(0)
+    layer = ss.StateSpaceLayer(16).to(DEV)
+    x, token = rand(4, 2, 16), rand(2, 16, seed=1)
+    conv, scan = rand(2, 3, 32, seed=2), rand(2, 32, 16, seed=3)
+    params = list(layer.parameters())
+    y, _ = layer(x, state=(conv, scan), return_state=True)
+    want = torch.autograd.grad(y.sum(), params)
+    y, _ = layer(x, state=(conv, scan), return_state=True)
+    layer.step(token, (conv.clone(), scan.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), params), want))
+    y, _ = layer(x, state=(conv, scan), return_state=True)
+    layer.step(token, (conv, scan))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

@@ -1,0 +1,28 @@
+"""State-space layer without a GPU: what the calls tell autograd, and what they refuse."""
+import pytest
+import torch
+
+from dfsnn_b200 import state_space as ss
+
+
+# ---------------------------------------------------------------------------------------
+# states written in place
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+def test_pool_written_in_place_raises_its_version(mode):
+    """As torch's own in-place operations, which count with gradients off too."""
+    state, out = torch.zeros(3, 4, 5), torch.zeros(3, 4, 5)
+    pool = torch.zeros(3, 2, 4, 5)
+    with mode():
+        for s, o, written in ((state, None, state), (state, out, out), (pool[:, 1], None, pool)):
+            before = written._version
+            ss._pool(s, o, torch.float32, -1, (4, 5), 3, None, "test")
+            assert written._version > before
+    assert state._version == 1                          # state_out leaves `state` as it was
+
+
+def test_pool_of_inference_tensors():
+    with torch.inference_mode():
+        state = torch.zeros(3, 4, 5)
+        ss._pool(state, None, torch.float32, -1, (4, 5), 3, None, "test")
+    ss._pool(state, None, torch.float32, -1, (4, 5), 3, None, "test")
