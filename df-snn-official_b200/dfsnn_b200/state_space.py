@@ -12,11 +12,11 @@ channels):
                    caller keeps (one for each row, or a pool with an index)
   StateSpaceLayer  the module around them: projections, convolution, scan
 
-The sequence forms are differentiable in every floating-point input.  Sequences are float32,
-float16 or bfloat16 (one type a call) with any strides over T and B, so halves of a projection
-and transposed batch-first tensors are read in place; outputs and gradients are dense in the
-order of the tensor they belong to.  Parameters, states and sums are float32.  There is no
-CPU path.
+The sequence forms are differentiable in every floating-point input (backwards; forward-mode
+tangents are refused).  Sequences are float32, float16 or bfloat16 (one type a call) with any
+strides over T and B, so halves of a projection and transposed batch-first tensors are read in
+place; outputs and gradients are dense in the order of the tensor they belong to.  Parameters,
+states and sums are float32.  There is no CPU path.
 
 All calls launch on the current stream of their tensors' device, wait for nothing and can be
 captured into a CUDA graph.  As with any torch operation, a backward can be captured only while
@@ -27,6 +27,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as _fw
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -156,6 +157,14 @@ def _pool(state, state_out, dtype, dev, inner, rows, index, name):
     if not state_out.is_inference():
         torch.autograd.graph.increment_version(state_out)
     return state_out, slots, stride, out_stride
+
+
+def _no_tangents(name, tensors):
+    """Refuses inputs with forward-mode tangents: they do not require a gradient, so a call would
+    pass them by and return a zero derivative."""
+    if _fw._current_level >= 0 and any(t is not None and _fw.unpack_dual(t).tangent is not None
+                                       for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode differentiation is not supported")
 
 
 # ---------------------------------------------------------------------------------------
@@ -295,6 +304,7 @@ def state_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=Fals
     h0 = _param(h0, dev, (Bn, Dn, N), name, "h0")
     lengths = _integers(lengths, dev, Bn, name, "lengths")
     tensors = (u, delta, A, B, C, D, z, bias, h0)
+    _no_tangents(name, tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         y, last = StateScanFunction.apply(*tensors, lengths, bool(softplus), bool(return_state))
     else:
@@ -326,6 +336,7 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
     D = _param(D, dev, (Dn,), name, "D")
     bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
     index = _integers(index, dev, Bn, name, "index")
+    _no_tangents(name, (u, delta, A, B, C, D, z, bias, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, torch.float32, dev, (Dn, N), Bn, index, name)
     y = u.new_empty(shape)
     args = _capi.STATE_SCAN_STEP_ARGS.pack(
@@ -415,6 +426,7 @@ def short_conv(x, weight, bias=None, activation=None, state=None, lengths=None, 
         state = _seq(state, x.dtype, dev, (Bn, W - 1, Dn), name, "state").contiguous()
     lengths = _integers(lengths, dev, Bn, name, "lengths")
     tensors = (x, weight, bias, state)
+    _no_tangents(name, tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         y, last = ShortConvFunction.apply(*tensors, lengths, silu, bool(return_state))
     else:
@@ -436,6 +448,7 @@ def short_conv_step(x, state, weight, bias=None, activation=None, index=None, st
     weight = _param(weight, dev, (Dn, W), name, "weight")
     bias = _param(bias, dev, (Dn,), name, "bias")
     index = _integers(index, dev, Bn, name, "index")
+    _no_tangents(name, (x, weight, bias, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, dtype, dev, (W - 1, Dn), Bn, index, name)
     y = x.new_empty(shape)
     args = _capi.SHORT_CONV_STEP_ARGS.pack(

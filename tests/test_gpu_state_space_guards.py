@@ -1,6 +1,7 @@
 """State-space layer on the GPU: calls that must not return a wrong answer silently."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from dfsnn_b200 import state_space as ss
 
@@ -54,3 +55,34 @@ def test_layer_step_on_a_saved_state_is_noticed():
     layer.step(token, (conv, scan))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+# ---------------------------------------------------------------------------------------
+# forward-mode tangents
+# ---------------------------------------------------------------------------------------
+def test_forward_mode_tangents_are_refused():
+    """Each input of each call in turn; the other inputs need gradients or not."""
+    T, B, D, N = 4, 2, 8, 4
+    scan = {"u": rand(T, B, D), "delta": rand(T, B, D, seed=1), "A": -rand(D, N).abs(), "B": rand(T, B, N),
+            "C": rand(T, B, N, seed=2), "D": rand(D), "z": rand(T, B, D, seed=3), "delta_bias": rand(D), "h0": rand(B, D, N)}
+    seqs = ("u", "delta", "B", "C", "z")
+    step = {k: v[0] if k in seqs else v for k, v in scan.items() if k != "h0"}
+    step["state"] = rand(B, D, N)
+    conv = {"x": rand(T, B, D), "weight": rand(D, 3), "bias": rand(D), "state": rand(B, 2, D)}
+    conv_step = {**conv, "x": conv["x"][0]}
+    for call, args in ((ss.state_scan, scan), (ss.state_scan_step, step), (ss.short_conv, conv),
+                       (ss.short_conv_step, conv_step)):
+        want = call(**{k: v.clone() for k, v in args.items()})
+        for k in args:
+            with forward_ad.dual_level():
+                got = call(**{n: v.clone() for n, v in args.items()})
+                assert torch.equal(got, want)
+                bad = {n: forward_ad.make_dual(v.clone(), torch.ones_like(v)) if n == k else v.clone()
+                       for n, v in args.items()}
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(**bad)
+                if call in (ss.state_scan, ss.short_conv):
+                    other = next(n for n in args if n != k)
+                    bad[other].requires_grad_(True)
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        call(**bad)

@@ -1,6 +1,7 @@
 """State-space layer without a GPU: what the calls tell autograd, and what they refuse."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from dfsnn_b200 import state_space as ss
 
@@ -26,3 +27,17 @@ def test_pool_of_inference_tensors():
         state = torch.zeros(3, 4, 5)
         ss._pool(state, None, torch.float32, -1, (4, 5), 3, None, "test")
     ss._pool(state, None, torch.float32, -1, (4, 5), 3, None, "test")
+
+
+# ---------------------------------------------------------------------------------------
+# forward-mode tangents
+# ---------------------------------------------------------------------------------------
+def test_forward_mode_tangents_are_refused():
+    x = torch.ones(3)
+    ss._no_tangents("test", (x, None))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        ss._no_tangents("test", (x, None))              # a level alone harms nobody
+        for tensors in ((dual,), (x, None, dual), (dual.double().contiguous(),)):
+            with pytest.raises(NotImplementedError, match="test: forward-mode"):
+                ss._no_tangents("test", tensors)
