@@ -167,6 +167,13 @@ def _no_tangents(name, tensors):
         raise NotImplementedError(f"{name}: forward-mode differentiation is not supported")
 
 
+def _no_gradients(name, tensors):
+    """Refuses what a step form could only cut off from its graph, as torch does for `out=`."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is not differentiable, but an input requires a gradient: call it under "
+                           "torch.no_grad(), or the sequence form with one step")
+
+
 # ---------------------------------------------------------------------------------------
 # calls
 # ---------------------------------------------------------------------------------------
@@ -314,7 +321,8 @@ def state_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=Fals
 
 def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, softplus=False,
                     index=None, state_out=None):
-    """One step of the selective scan for each of B rows; not differentiable.
+    """One step of the selective scan for each of B rows; not differentiable (refused where an input
+    requires a gradient and gradients are enabled).
 
     u, delta, z [B, D]; B, C [B, N] or [B, G, N]; state float32 [S, D, N], a slot for each row
     or, with index (int32 / int64 [B], on the device), a pool of S slots of which row b uses
@@ -336,7 +344,9 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
     D = _param(D, dev, (Dn,), name, "D")
     bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
     index = _integers(index, dev, Bn, name, "index")
-    _no_tangents(name, (u, delta, A, B, C, D, z, bias, state))
+    tensors = (u, delta, A, B, C, D, z, bias)
+    _no_gradients(name, tensors)
+    _no_tangents(name, (*tensors, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, torch.float32, dev, (Dn, N), Bn, index, name)
     y = u.new_empty(shape)
     args = _capi.STATE_SCAN_STEP_ARGS.pack(
@@ -435,7 +445,7 @@ def short_conv(x, weight, bias=None, activation=None, state=None, lengths=None, 
 
 
 def short_conv_step(x, state, weight, bias=None, activation=None, index=None, state_out=None):
-    """One step of the short convolution for each of B rows; not differentiable.
+    """One step of the short convolution for each of B rows; not differentiable (as state_scan_step).
 
     x [B, D]; state [S, W - 1, D], x's type: the last inputs of each slot, oldest first, as
     short_conv returns them; index and state_out as in state_scan_step.  Returns y [B, D]."""
@@ -448,6 +458,7 @@ def short_conv_step(x, state, weight, bias=None, activation=None, index=None, st
     weight = _param(weight, dev, (Dn, W), name, "weight")
     bias = _param(bias, dev, (Dn,), name, "bias")
     index = _integers(index, dev, Bn, name, "index")
+    _no_gradients(name, (x, weight, bias))
     _no_tangents(name, (x, weight, bias, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, dtype, dev, (W - 1, Dn), Bn, index, name)
     y = x.new_empty(shape)

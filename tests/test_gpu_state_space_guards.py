@@ -86,3 +86,24 @@ def test_forward_mode_tangents_are_refused():
                     bad[other].requires_grad_(True)
                     with pytest.raises(NotImplementedError, match="forward-mode"):
                         call(**bad)
+
+
+# ---------------------------------------------------------------------------------------
+# gradients through the step forms
+# ---------------------------------------------------------------------------------------
+def test_steps_refuse_inputs_that_require_gradients():
+    """They could only return outputs cut off from the graph.  Nothing is written before the refusal."""
+    B, D, N = 2, 8, 4
+    scan = {"u": rand(B, D), "delta": rand(B, D, seed=1), "A": -rand(D, N).abs(), "B": rand(B, N),
+            "C": rand(B, N, seed=2), "D": rand(D), "z": rand(B, D, seed=3), "delta_bias": rand(D)}
+    conv = {"x": rand(B, D), "weight": rand(D, 3), "bias": rand(D)}
+    for call, args, state in ((ss.state_scan_step, scan, rand(B, D, N)), (ss.short_conv_step, conv, rand(B, 2, D))):
+        want = call(**args, state=state.clone())
+        for k in args:
+            leaves = {n: v.detach().requires_grad_(n == k) for n, v in args.items()}
+            kept = state.clone()
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                call(**leaves, state=kept)
+            assert torch.equal(kept, state) and kept._version == 0
+            with torch.no_grad():
+                assert torch.equal(call(**leaves, state=kept), want)

@@ -41,3 +41,15 @@ def test_forward_mode_tangents_are_refused():
         for tensors in ((dual,), (x, None, dual), (dual.double().contiguous(),)):
             with pytest.raises(NotImplementedError, match="test: forward-mode"):
                 ss._no_tangents("test", tensors)
+
+
+# ---------------------------------------------------------------------------------------
+# gradients through the step forms
+# ---------------------------------------------------------------------------------------
+def test_steps_refuse_inputs_that_require_gradients():
+    x, w = torch.ones(3), torch.ones(3, requires_grad=True)
+    ss._no_gradients("test", (x, None))
+    with torch.no_grad():
+        ss._no_gradients("test", (x, w))
+    with pytest.raises(RuntimeError, match="test is not differentiable"):
+        ss._no_gradients("test", (x, None, w))
