@@ -478,9 +478,11 @@ class StateSpaceLayer(nn.Module):
     """Projections, short convolution and gated selective scan: [T, B, d_model] -> the same.
 
     step_mode 'm' takes a whole sequence a call, 's' one step [B, d_model] a call, carrying its
-    states until reset(), as the neurons do.  Serving code that keeps its own states uses
-    forward(..., state=, return_state=True) for prompts and step() for tokens: a state is the
-    pair (convolution inputs [S, taps - 1, d_inner], scan states [S, d_inner, d_state])."""
+    states until reset().  Where gradients are enabled and asked for, the steps are differentiable:
+    the carried states are part of the graph, which goes back to the last reset() (or to the last
+    step without gradients).  Serving code that keeps its own states uses
+    forward(..., state=, return_state=True) for prompts and step() for tokens: a state is the pair
+    (convolution inputs [S, taps - 1, d_inner], scan states [S, d_inner, d_state])."""
 
     def __init__(self, d_model, d_state=16, taps=4, expand=2, groups=1, rank=None, step_mode="m",
                  step_range=(1e-3, 1e-1)):
@@ -526,7 +528,10 @@ class StateSpaceLayer(nn.Module):
         if self.step_mode == "s":
             if lengths is not None or state is not None or return_state:
                 raise ValueError("step_mode 's' carries its own state: use step()")
-            return self.step(x, self._state)
+            return self._carried_step(x)
+        return self._sequence(x, lengths, state, return_state)
+
+    def _sequence(self, x, lengths, state, return_state):
         conv0, h0 = (None, None) if state is None else state
         x, z = self.in_proj(x).chunk(2, dim=-1)
         x = short_conv(x, self.conv_weight, self.conv_bias, "silu", conv0, lengths, return_state)
@@ -540,9 +545,21 @@ class StateSpaceLayer(nn.Module):
         y = self.out_proj(y)
         return (y, (conv0, h0)) if return_state else y
 
+    def _carried_step(self, x):
+        state = self._state
+        if state is not None and state[1].shape[0] != x.shape[0]:
+            raise ValueError(f"step_mode 's': the carried states are those of {state[1].shape[0]} rows, got "
+                             f"{x.shape[0]}: call reset() before another batch")
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *self.parameters(), *(state or ()))):
+            y, self._state = self._sequence(x.unsqueeze(0), None, state, True)
+            return y.squeeze(0)
+        if state is not None:                   # of a step with gradients: nothing saved them yet
+            state = self._state = tuple(s.detach() for s in state)
+        return self.step(x, state)
+
     @torch.no_grad()
     def step(self, x, state, index=None):
-        """One token for each row of x [B, d_model]; state is advanced in place."""
+        """One token for each row of x [B, d_model], without gradients; state is advanced in place."""
         x, z = self.in_proj(x).chunk(2, dim=-1)
         if state is None:                       # the layer's own, from zero
             state = self._state = self.initial_state(x.shape[0], x.dtype, x.device)

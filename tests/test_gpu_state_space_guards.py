@@ -107,3 +107,56 @@ def test_steps_refuse_inputs_that_require_gradients():
             assert torch.equal(kept, state) and kept._version == 0
             with torch.no_grad():
                 assert torch.equal(call(**leaves, state=kept), want)
+
+
+# ---------------------------------------------------------------------------------------
+# the layer, step by step
+# ---------------------------------------------------------------------------------------
+def test_layer_in_single_steps_has_the_gradients_of_the_sequence():
+    """Outputs and every gradient of T single steps against 64 bits.  Every path has a few hundred
+    roundings (T steps of the scan, sums over 96 channels, T B rows) and four projections with sums of
+    at most 96 terms; norm against norm, the bounds of the whole sequence's test."""
+    from test_gpu_state_space import layer_64
+    torch.manual_seed(0)
+    T, B = 7, 3
+    layer = ss.StateSpaceLayer(48, groups=2, step_mode="s").to(DEV)
+    x = rand(T, B, 48).requires_grad_(True)
+    gy = rand(T, B, 48, seed=1)
+    rel = lambda a, b: float((a.detach().double() - b.detach()).norm() / b.detach().norm())  # noqa: E731
+    for _ in range(2):                                   # reset() starts anew
+        y = torch.stack([layer(x[t]) for t in range(T)])
+        x64 = x.detach().double().requires_grad_(True)
+        y64, p = layer_64(layer, x64)
+        got = torch.autograd.grad(y, [x, *layer.parameters()], gy)
+        want = torch.autograd.grad(y64, [x64, *p.values()], gy.double())
+        assert rel(y, y64) < 2000 * 2.0 ** -24
+        for k, a, b in zip(("x", *p), got, want):
+            assert rel(a, b) < 20000 * 2.0 ** -24, k
+        layer.reset()
+    # steps without gradients go on from those with, in place, and the other way round
+    y = [layer(x[0])]
+    with torch.no_grad():
+        y += [layer(x[1])]
+        carried = layer._state[1].data_ptr()
+        y += [layer(x[2])]
+        assert not y[-1].requires_grad and layer._state[1].data_ptr() == carried
+    y += [layer(x[3])]
+    assert rel(torch.stack(y), y64[:4].detach()) < 2000 * 2.0 ** -24
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(y[3].sum() + y[0].sum(), list(layer.parameters())))
+
+
+def test_layer_refuses_a_batch_that_is_not_the_carried_one():
+    layer = ss.StateSpaceLayer(16, step_mode="s").to(DEV)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode():
+            layer.reset()
+            layer(rand(8, 16))
+            kept = [s.detach().clone() for s in layer._state]
+            for x in (rand(4, 16), rand(9, 16)):
+                with pytest.raises(ValueError, match="call reset"):
+                    layer(x)
+            with pytest.raises((ValueError, RuntimeError)):      # another type
+                layer(rand(8, 16).double())
+            assert all(torch.equal(a, b) for a, b in zip(kept, layer._state))
+            layer.reset()
+            assert layer(rand(4, 16)).shape == (4, 16)
