@@ -47,7 +47,10 @@ struct Tile {
     float2 d[BC][TT + 1];                            // (d, d u)
     float g[BC][TT + 1];                             // grad o
     float lb[BC][TT + 1], qa[BC][TT + 1], o[BC][TT + 1];    // sums over states
-    float sums[2][NT];
+    // a thread's sums of grad A (pairs of states) and of grad D and delta_bias (a pack's channels),
+    // added to after every tile: one fp32 register each for the many steps of many sequences that a
+    // block takes lost digits (16 steps, 4096 sequences: grad A 4.2e-7 from 64 bits, now 2.1e-7)
+    __align__(16) double2 sum_a[C * S / 2][NT], sum_d[2][NT];
     int ready;
 };
 
@@ -67,6 +70,9 @@ __device__ __forceinline__ void store_states(float* q, const float (&v)[S][Q], i
     else *reinterpret_cast<float2*>(q) = make_float2(v[0][i], v[1][i]);
 }
 __device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+__device__ __forceinline__ void add_to(double2& sum, float2 v) {
+    sum = make_double2(sum.x + v.x, sum.y + v.y);
+}
 
 // V neighbouring elements of a sequence
 template <typename IO, int V>
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
     const int ch = tid % ROW * V, t_e = tid / ROW;
     const bool ch_ok = ch < cols && t_e < TT;
     const long long chan = g_base + c_base + ch;
-    float2 bias = two(0.0f), skip = two(0.0f), sum_D = two(0.0f), sum_bias = two(0.0f);
+    float2 bias = two(0.0f), skip = two(0.0f);
     if (ch_ok && a.delta_bias) bias = make_float2(a.delta_bias[chan], a.delta_bias[chan + V - 1]);
     if (ch_ok && a.D) skip = make_float2(a.D[chan], a.D[chan + V - 1]);
 
@@ -170,7 +176,10 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
             for (int s = 0; s < S; ++s)
                 if (cl + c * CL < cols && n0 + s < a.states) q[c * crow + s] = s % 2 ? v[c][s / 2].y : v[c][s / 2].x;
     };
-    float2 A2[C][J] = {}, dA[C][J] = {};
+    // each thread has its own; the first use by others is behind a barrier
+    for (int i = 0; i < C * J; ++i) sh.sum_a[i][tid] = make_double2(0.0, 0.0);
+    for (int i = 0; i < 2; ++i) sh.sum_d[i][tid] = make_double2(0.0, 0.0);
+    float2 A2[C][J] = {};
     get(a.A + (g_base + c_base + cl) * a.states + n0, A2);
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -317,6 +326,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                     near1[c][j] = most * fmaxf(fabsf(A2[c][j].x), fabsf(A2[c][j].y)) < kExp2Near;
             }
 
+            float2 dA[C][J] = {};
 #pragma unroll 1
             for (int tr = TT - R; tr >= 0; tr -= R) {
                 if (t0 + tr >= len) continue;
@@ -426,10 +436,15 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                     over_channels(dB, sh.red[warp][0], tq);
                 }
             }
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int j = 0; j < J; ++j) add_to(sh.sum_a[c * J + j][tid], dA[c][j]);
             __syncthreads();
 
             // elementwise gradients
             if (ch_ok) {
+                float2 sum_D = two(0.0f), sum_bias = two(0.0f);
                 IO *gu_t = gu_p + t0 * g.gu_t, *gd_t = gd_p + t0 * g.gdelta_t, *gz_t = gz_p + t0 * g.gz_t;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
@@ -459,6 +474,8 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                         sum_D = __ffma2_rn(go, tail && t0 + t >= len ? two(0.0f) : u, sum_D);
                     }
                 }
+                add_to(sh.sum_d[0][tid], sum_D);
+                add_to(sh.sum_d[1][tid], sum_bias);
             }
             // this block's part of grad B and grad C
 #pragma unroll
@@ -492,22 +509,25 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
         __syncthreads();                                        // before the next sequence's copies
     }
 
-    put(p.part_a + ((long long)part * a.channels + g_base + c_base + cl) * a.states + n0, dA);
-    // the threads of a channel, in order
+    float2 dA[C][J];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        __syncthreads();
-        sh.sums[0][tid] = v ? sum_D.y : sum_D.x;
-        sh.sums[1][tid] = v ? sum_bias.y : sum_bias.x;
-        __syncthreads();
-        if (tid < ROW && ch + v < cols) {
-            float d = 0.0f, e = 0.0f;
-            for (int i = tid; i < NT; i += ROW) {
-                d += sh.sums[0][i];
-                e += sh.sums[1][i];
-            }
-            p.part_d[(long long)part * a.channels + chan + v] = d;
-            p.part_d[((long long)parts + part) * a.channels + chan + v] = e;
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const double2 v = sh.sum_a[c * J + j][tid];
+            dA[c][j] = make_float2((float)v.x, (float)v.y);
+        }
+    put(p.part_a + ((long long)part * a.channels + g_base + c_base + cl) * a.states + n0, dA);
+    // the threads of a pack's channels, in order
+    __syncthreads();
+    if (tid < ROW) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            double2 v = make_double2(0.0, 0.0);
+            for (int i = tid; i < NT; i += ROW) v = make_double2(v.x + sh.sum_d[which][i].x, v.y + sh.sum_d[which][i].y);
+            float* q = p.part_d + ((long long)which * parts + part) * a.channels + chan;
+            if (ch < cols) q[0] = (float)v.x;
+            if (V == 2 && ch + 1 < cols) q[1] = (float)v.y;
         }
     }
 }
@@ -672,7 +692,7 @@ __global__ void __launch_bounds__(kSumThreads) scan_bwd_sums(const ScanParams p,
         else add(std::integral_constant<int, 1>{});
         return;
     }
-    __shared__ float s_sum[kSumThreads / 32][32];
+    __shared__ double s_sum[kSumThreads / 32][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long i = (long long)(blockIdx.x - bc_blocks) * 32 + lane;
     const int parts = p.batch_parts * p.splits;
@@ -690,7 +710,7 @@ __global__ void __launch_bounds__(kSumThreads) scan_bwd_sums(const ScanParams p,
         out = which ? g.grad_delta_bias : g.grad_D;
         if (out) out += c;
     }
-    float v = 0.0f;
+    double v = 0.0;
     if (out) {
 #pragma unroll 4
         for (int j = warp; j < parts; j += kSumThreads / 32) v += q[j * stride];
@@ -698,9 +718,9 @@ __global__ void __launch_bounds__(kSumThreads) scan_bwd_sums(const ScanParams p,
     s_sum[warp][lane] = v;
     __syncthreads();
     if (warp == 0 && out) {
-        v = 0.0f;
+        v = 0.0;
         for (int w = 0; w < kSumThreads / 32; ++w) v += s_sum[w][lane];
-        *out = v;
+        *out = (float)v;
     }
 }
 
@@ -722,6 +742,7 @@ cudaError_t launch_form(const ScanParams& p, cudaStream_t st) {
         scan_bwd_ends<IO, S, SL, WIDE><<<(unsigned)n, NT, sizeof(Ends), st>>>(q);
     }
     constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
+    static_assert(S * SL > 64 || 3 * (smem + 1024) <= 228 * 1024, "three blocks an SM up to 64 states");
     cudaError_t e = allow_shared<scan_bwd<IO, S, SL, C, WIDE>>(smem);
     if (e != cudaSuccess) return e;
     scan_bwd<IO, S, SL, C, WIDE><<<(unsigned)blocks, NT, smem, st>>>(p);
