@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < J; ++j) A2[c][j] = __fmul2_rn(A2[c][j], two(kLog2e));
+        for (int j = 0; j < J; ++j) A2[c][j] = make_float2(log2_rate(A2[c][j].x), log2_rate(A2[c][j].y));
 
     for (long long b = batch_part; b < a.batch; b += p.batch_parts) {
         const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T);
@@ -579,8 +579,8 @@ __global__ void __launch_bounds__(NT) scan_bwd_ends(const ScanParams p) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const bool ok = cl < cols;
-        A2[j].x = ok && n0 + 2 * j < a.states ? a.A[ch_row * a.states + n0 + 2 * j] * kLog2e : 0.0f;
-        A2[j].y = ok && n0 + 2 * j + 1 < a.states ? a.A[ch_row * a.states + n0 + 2 * j + 1] * kLog2e : 0.0f;
+        A2[j].x = ok && n0 + 2 * j < a.states ? log2_rate(a.A[ch_row * a.states + n0 + 2 * j]) : 0.0f;
+        A2[j].y = ok && n0 + 2 * j + 1 < a.states ? log2_rate(a.A[ch_row * a.states + n0 + 2 * j + 1]) : 0.0f;
     }
     float steps = 0.0f;
     auto fill = [&](int t0) {

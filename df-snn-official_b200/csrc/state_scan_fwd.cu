@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-        for (int j = 0; j < S / 2; ++j) A2[c][j] = make_float2(A2[c][j].x * kLog2e, A2[c][j].y * kLog2e);
+        for (int j = 0; j < S / 2; ++j) A2[c][j] = make_float2(log2_rate(A2[c][j].x), log2_rate(A2[c][j].y));
 
     for (long long b = b0; b < a.batch; b += p.seq_blocks) {
     const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T), len = whole_len < stop ? whole_len : stop;

@@ -2,6 +2,7 @@
 // causal convolution, and their single-token forms).
 #pragma once
 #include <atomic>
+#include <cfloat>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -73,6 +74,14 @@ __device__ __forceinline__ float2 exp2_near1(float2 x) {
     float2 q = __ffma2_rn(x, make_float2(0.0555093173f, 0.0555093173f), make_float2(0.2402546865f, 0.2402546865f));
     q = __ffma2_rn(x, q, make_float2(0.693147178f, 0.693147178f));
     return __ffma2_rn(x, q, one);
+}
+
+// A log2 e, as the scans keep it.  An infinite product becomes the largest number: a step behind the
+// end has d = 0 and leaves the state alone (0 times infinity would not), and any other d still gives
+// the decay 0 (or infinity).
+__device__ __forceinline__ float log2_rate(float a) {
+    a *= kLog2e;
+    return isinf(a) ? copysignf(FLT_MAX, a) : a;
 }
 
 // sequence length of row b: lengths[b] clamped to [0, T]; T without lengths

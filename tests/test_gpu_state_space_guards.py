@@ -3,7 +3,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import state_ref
 from dfsnn_b200 import state_space as ss
+from test_gpu_state_space import close, scan_case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -160,3 +162,28 @@ def test_layer_refuses_a_batch_that_is_not_the_carried_one():
             assert all(torch.equal(a, b) for a, b in zip(kept, layer._state))
             layer.reset()
             assert layer(rand(4, 16)).shape == (4, 16)
+
+
+# ---------------------------------------------------------------------------------------
+# values at the ends of the range
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,B,D,N,G,lengths", [
+    (17, 2, 40, 16, 1, None), (16, 3, 33, 5, 1, [16, 7, 0]), (40, 4, 24, 40, 2, [40, 1, 0, 23]), (31, 2, 9, 100, 1, None),
+    (9, 2, 40, 8, 1, [3, 9]), (900, 1, 20, 16, 1, None), (901, 2, 12, 3, 1, [900, 461]), (300, 480, 8, 16, 1, None)])
+def test_scan_states_that_forget_at_once(T, B, D, N, G, lengths):
+    """A = -inf: the decay is 0, on a step behind a sequence's end (or in the rest of a tile) as well as
+    on any other, where it must not touch the state.  The formula with -1e30 in its place has the same
+    values.  A decay of 0 has no error, so the bound goes by the other states (as in test_scan_*)."""
+    x, n, (gy, gh) = scan_case(T, B, D, N, G, "f32", lengths=lengths, seed=T, scale=0.1)
+    x["A"][:, ::3] = -float("inf")
+    leaves = {k: v.detach().requires_grad_(True) for k, v in x.items()}
+    y, h = ss.state_scan(**leaves, softplus=True, lengths=n, return_state=True)
+    got = dict(zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [gy, gh])))
+    ref = {**x, "A": x["A"].clamp_min(-1e30)}
+    want, mag = (state_ref.scan(**ref, softplus=True, lengths=n, gy=gy, gh=gh, mag=m) for m in (False, True))
+    m = state_ref.scan(**{**x, "A": x["A"].nan_to_num(neginf=0.0)}, softplus=True, lengths=n)["step_decay"]
+    K = 2 * T * (10 * m + 6) + N + D + T * B + 2 * float(x["z"].nan_to_num().abs().max()) + 60
+    close(y, want["y"], mag["y"], K, ("y", y.dtype))
+    close(h, want["h"], mag["h"], K, ("h", h.dtype))
+    for k, v in got.items():
+        close(v, want["g" + k], mag["g" + k], K, ("grad " + k, v.dtype))
