@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                     const float d = cl + c * CL < cols ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
 #pragma unroll
                     for (int j = 0; j < J; ++j)
-                        lam[c][j] = make_float2(fmaf(exp2_approx(d * A2[c][j].x), lam[c][j].x, end[c][j].x),
-                                                fmaf(exp2_approx(d * A2[c][j].y), lam[c][j].y, end[c][j].y));
+                        lam[c][j] = make_float2(carry_over(d * A2[c][j].x, lam[c][j].x, end[c][j].x),
+                                                carry_over(d * A2[c][j].y, lam[c][j].y, end[c][j].y));
                 }
             }
         }

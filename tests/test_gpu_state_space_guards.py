@@ -187,3 +187,44 @@ def test_scan_states_that_forget_at_once(T, B, D, N, G, lengths):
     close(h, want["h"], mag["h"], K, ("h", h.dtype))
     for k, v in got.items():
         close(v, want["g" + k], mag["g" + k], K, ("grad " + k, v.dtype))
+
+
+def test_scan_parts_whose_decay_overflows():
+    """A > 0 in few long sequences, walked in parts of 64 steps: over a part the decay (up to e^96, e^128)
+    is more than a float holds, the states are not.  Zero states stay zero, small ones grow; and the same
+    for the gradients.  Bounds as in test_gpu_state_space.py; a part's decay is off by the rounding of its
+    exponent, which is less than its steps' together."""
+    T, D, N = 1024, 32, 16
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(len(s))).to(DEV)  # noqa: E731
+    A = (2.9 + 0.1 * torch.rand(D, N, generator=torch.Generator().manual_seed(1))).to(DEV)
+    B, C, delta = r(T, 1, 1, N), r(T, 1, 1, N).flip(0), torch.full((T, 1, D), 1e-3, device=DEV)
+    K = 2 * T * (10 * 1.5 + 6) + N + D + T + 60
+
+    def check(u, delta, h0, gy):
+        x = {"u": u, "delta": delta, "A": A, "B": B, "C": C, "h0": h0}
+        leaves = {k: v.clone().requires_grad_(True) for k, v in x.items()}
+        y, h = ss.state_scan(**leaves, return_state=True)
+        got = () if gy is None else torch.autograd.grad(y, list(leaves.values()), gy)
+        want, mag = (state_ref.scan(**x, gy=gy, mag=m) for m in (False, True))
+        names = [(y, "y"), (h, "h"), *((v, "g" + k) for k, v in zip(leaves, got))]
+        assert all(float(want[k].abs().max()) < 1e30 for _, k in names)
+        assert max(float(want[k].abs().max()) for _, k in names) > 0
+        for v, k in names:
+            close(v, want[k], mag[k], K, (k, v.dtype))
+
+    # nothing before step 900, long steps until then (whose gradients would be infinite)
+    u, d = r(T, 1, D), delta.clone()
+    u[:900], d[:900] = 0, 0.5
+    check(u, d, torch.zeros(1, D, N, device=DEV), None)
+    # a small state that grows in the first part
+    d = delta.clone()
+    d[:64] = 0.5
+    check(torch.zeros(T, 1, D, device=DEV), d, torch.full((1, D, N), 1e-30, device=DEV), torch.zeros(T, 1, D, device=DEV))
+    # no gradient from the long steps at the end; no states either
+    d, gy = delta.clone(), r(T, 1, D)
+    d[100:], gy[100:] = 0.5, 0
+    check(torch.zeros(T, 1, D, device=DEV), d, torch.zeros(1, D, N, device=DEV), gy)
+    # a small gradient that grows in the last part
+    d, gy = delta.clone(), torch.zeros(T, 1, D, device=DEV)
+    d[-64:], gy[-1] = 0.5, 1e-30
+    check(torch.zeros(T, 1, D, device=DEV), d, torch.zeros(1, D, N, device=DEV), gy)
