@@ -256,11 +256,11 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                 get(p.ends + k * rows * a.states + row, end);
 #pragma unroll
                 for (int c = 0; c < C; ++c) {
-                    const float d = cl + c * CL < cols ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
+                    const float half = cl + c * CL < cols ? 0.5f * p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
 #pragma unroll
                     for (int j = 0; j < J; ++j)
-                        lam[c][j] = make_float2(carry_over(d * A2[c][j].x, lam[c][j].x, end[c][j].x),
-                                                carry_over(d * A2[c][j].y, lam[c][j].y, end[c][j].y));
+                        lam[c][j] = make_float2(carry_over(half * A2[c][j].x, lam[c][j].x, end[c][j].x),
+                                                carry_over(half * A2[c][j].y, lam[c][j].y, end[c][j].y));
                 }
             }
         }

@@ -214,11 +214,11 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
             get(p.ends + k * rows * a.states + row, end);
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const float d = cl_ok(c) ? p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
+                const float half = cl_ok(c) ? 0.5f * p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
 #pragma unroll
                 for (int j = 0; j < S / 2; ++j)
-                    h[c][j] = make_float2(carry_over(d * A2[c][j].x, h[c][j].x, end[c][j].x),
-                                          carry_over(d * A2[c][j].y, h[c][j].y, end[c][j].y));
+                    h[c][j] = make_float2(carry_over(half * A2[c][j].x, h[c][j].x, end[c][j].x),
+                                          carry_over(half * A2[c][j].y, h[c][j].y, end[c][j].y));
             }
         }
     } else if (split == 0) {

@@ -84,13 +84,12 @@ __device__ __forceinline__ float log2_rate(float a) {
     return isinf(a) ? copysignf(FLT_MAX, a) : a;
 }
 
-// 2^x h + end, where 2^x is the decay over a whole part of a sequence.  Step by step a growing state
-// stays finite as long as it is; 2^x alone need not (nor is 0 times its infinity 0), so the
-// power's whole part goes to the product's exponent.
+// 2^(2 x) h + end, where 2^(2 x) is the decay over a whole part of a sequence.  Step by step a growing
+// state stays finite as long as it is; the power alone need not (nor is 0 times its infinity 0), so it
+// is taken as two factors.  (A NaN in x is one in `end` too.)
 __device__ __forceinline__ float carry_over(float x, float h, float end) {
-    x = x > 400.0f ? 400.0f : x < -400.0f ? -400.0f : x;       // everything is infinite, or 0, by then
-    const float n = rintf(x);
-    return scalbnf(exp2_approx(x - n) * h, (int)n) + end;
+    const float f = exp2_approx(fminf(x, 127.5f));              // any state overflows by 2^255
+    return fmaf(f * h, f, end);
 }
 
 // sequence length of row b: lengths[b] clamped to [0, T]; T without lengths
