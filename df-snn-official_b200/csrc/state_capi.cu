@@ -51,6 +51,7 @@ dfsnn::ScanParams scan_params(const dfsnn_state_scan_args& a) {
     p.group_channels = (int)(a.channels / a.groups);
     p.splits = 1;
     p.split_steps = p.T;
+    p.patience = 1;
     return p;
 }
 
@@ -71,6 +72,30 @@ ScanWorkspace backward_plan(dfsnn::ScanParams& p) {
     w.end_steps = p.splits > 1 && !p.chained ? p.splits * rows : 0;
     w.flags = p.chained ? (size_t)p.tiles * p.a.groups * p.batch_parts + 1 : 0;
     return w;
+}
+
+int backward(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g, void* workspace,
+             size_t workspace_bytes, int patience, void* stream) {
+    if (int s = check_scan(a)) return s;
+    if (!g) return DFSNN_ERR_NULL;
+    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
+    if (!a->u || !a->delta || !a->A || !a->B || !a->C || !g->grad_y || !g->grad_u || !g->grad_delta
+        || !g->grad_B || !g->grad_C || !g->grad_A)
+        return DFSNN_ERR_NULL;
+    if (!a->kept && a->T > DFSNN_SCAN_CHUNK) return DFSNN_ERR_NULL;
+    dfsnn::ScanParams p = scan_params(*a);
+    p.g = *g;
+    p.patience = patience;
+    const ScanWorkspace w = backward_plan(p);
+    if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return DFSNN_ERR_WORKSPACE;
+    p.part_bc = static_cast<float*>(workspace);
+    p.part_a = p.part_bc + w.bc;
+    p.part_d = p.part_a + w.a;
+    p.ends = p.part_d + w.d;
+    p.end_steps = p.ends + w.ends;
+    p.flags = reinterpret_cast<int*>(p.end_steps + w.end_steps);
+    p.places = p.flags + (w.flags ? w.flags - 1 : 0);
+    return status(dfsnn::state_scan_backward_launch(p, (cudaStream_t)stream));
 }
 
 }  // namespace
@@ -138,25 +163,17 @@ int dfsnn_state_scan_backward_launches(long long T, long long batch, long long c
 
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g,
                               void* workspace, size_t workspace_bytes, void* stream) {
-    if (int s = check_scan(a)) return s;
-    if (!g) return DFSNN_ERR_NULL;
-    if (a->batch == 0 || a->channels == 0) return DFSNN_OK;
-    if (!a->u || !a->delta || !a->A || !a->B || !a->C || !g->grad_y || !g->grad_u || !g->grad_delta
-        || !g->grad_B || !g->grad_C || !g->grad_A)
-        return DFSNN_ERR_NULL;
-    if (!a->kept && a->T > DFSNN_SCAN_CHUNK) return DFSNN_ERR_NULL;
-    dfsnn::ScanParams p = scan_params(*a);
-    p.g = *g;
-    const ScanWorkspace w = backward_plan(p);
-    if (!workspace || !aligned16(workspace) || workspace_bytes < w.bytes()) return DFSNN_ERR_WORKSPACE;
-    p.part_bc = static_cast<float*>(workspace);
-    p.part_a = p.part_bc + w.bc;
-    p.part_d = p.part_a + w.a;
-    p.ends = p.part_d + w.d;
-    p.end_steps = p.ends + w.ends;
-    p.flags = reinterpret_cast<int*>(p.end_steps + w.end_steps);
-    p.error = p.flags + (w.flags ? w.flags - 1 : 0);
-    return status(dfsnn::state_scan_backward_launch(p, (cudaStream_t)stream));
+    return backward(a, g, workspace, workspace_bytes, 1, stream);
+}
+
+int dfsnn_check_state_scan_waits(const dfsnn_state_scan_args* a, const dfsnn_state_scan_grads* g,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+    return backward(a, g, workspace, workspace_bytes, 0, stream);
+}
+
+int dfsnn_state_scan_expired_waits(unsigned long long* count, void* stream) {
+    if (!count) return DFSNN_ERR_NULL;
+    return status(dfsnn::state_scan_expired_waits(count, (cudaStream_t)stream));
 }
 
 int dfsnn_state_scan_step(const dfsnn_state_scan_step_args* a, void* stream) {

@@ -20,7 +20,8 @@ struct ScanParams {
     float* end_steps;                          // the last, backward: the first unused) and sums of d
     int chained;                               // backward: the parts run in order, `ends` passed on
     int* flags;                                // [tiles * groups * batch] finished parts, zeroed first
-    int* error;                                // behind them: a wait that ran out
+    int* places;                               // behind them: places given to blocks so far
+    int patience;                              // 1; 0: every wait runs out at once (self-check)
     // backward
     int batch_parts;                           // blocks that share the batch (part q: b = q, q + parts, ...)
     float* part_bc;                            // [2][tiles][T][batch][groups][states]
@@ -51,5 +52,6 @@ cudaError_t state_scan_forward_launch(const ScanParams& p, cudaStream_t st);
 int state_scan_bwd_tiles(int states, long long group_channels);
 void state_scan_bwd_plan(ScanParams& p);       // sets splits, split_steps and batch_parts
 cudaError_t state_scan_backward_launch(const ScanParams& p, cudaStream_t st);
+cudaError_t state_scan_expired_waits(unsigned long long* count, cudaStream_t st);
 
 }  // namespace dfsnn

@@ -51,7 +51,7 @@ struct Tile {
     // added to after every tile: one fp32 register each for the many steps of many sequences that a
     // block takes lost digits (16 steps, 4096 sequences: grad A 4.2e-7 from 64 bits, now 2.1e-7)
     __align__(16) double2 sum_a[C * S / 2][NT], sum_d[2][NT];
-    int ready;
+    int place, ready;
 };
 
 template <int S>
@@ -92,17 +92,20 @@ __device__ __forceinline__ void store(IO* q, float2 f) {
     *reinterpret_cast<Pack<IO, V>*>(q) = p;
 }
 
-// The flag of a chain counts its finished parts.  A wait ends after some seconds at the latest: then
-// the error word is set and the caller goes on with NaN, which reaches all that depends on it.
-constexpr unsigned kMaxPolls = 1u << 21;
-__device__ __forceinline__ bool wait_at_least(const int* flag, int count, int* error) {
-    for (unsigned i = 0; i < kMaxPolls; ++i) {
+// The flag of a chain counts its finished parts.  A part can take as long as the `steps` behind it
+// together (0.4 us a step); a poll takes 0.5 us at least, and a wait has 2^21 polls and 16 for each step.
+// A wait that runs out all the same is counted, and the caller goes on with NaN, which reaches all that
+// depends on it.
+__device__ unsigned long long expired_waits;
+__device__ __forceinline__ bool wait_at_least(const int* flag, int count, long long steps, int patience) {
+    const long long polls = patience * ((1LL << 21) + 16 * steps);
+    for (long long i = 0; i < polls; ++i) {
         int v;
         asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
         if (v >= count) return true;
         __nanosleep(200);
     }
-    *error = 1;
+    atomicAdd(&expired_waits, 1ULL);
     return false;
 }
 __device__ __forceinline__ void publish(int* flag, int count) {
@@ -123,13 +126,19 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
     const dfsnn_state_scan_grads& g = p.g;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    long long bid = blockIdx.x;
-    const long long chains = (long long)p.tiles * a.groups * p.batch_parts;
-    const long long chain = p.chained ? bid % chains : 0;       // (tile, group, sequence)
+    unsigned bid = blockIdx.x;
+    unsigned chain = 0;                                         // (tile, group, sequence)
     int split = 0;
-    if (p.chained) {                                            // all last parts, then all last but one, ...
+    if (p.chained) {
+        // Places in the order in which the blocks start: all last parts, then all last but one, ...  A
+        // part waits only for the next one of its sequence, whose place is in front of its own: that
+        // block runs or has run.
+        const unsigned chains = p.tiles * a.groups * p.batch_parts;
+        if (tid == 0) sh.place = atomicAdd(p.places, 1);
+        __syncthreads();
+        bid = __reduce_max_sync(0xffffffffu, (unsigned)sh.place);      // one value for the warp, in a uniform register
         split = p.splits - 1 - (int)(bid / chains);
-        bid = chain;
+        bid = chain = bid % chains;
     }
     const int tile = (int)(bid % p.tiles);
     bid /= p.tiles;
@@ -239,8 +248,7 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
         float2 lam[C][J] = {};                                  // a_(t+1) l_(t+1)
         const long long rows = a.batch * a.channels;
         if (p.chained && len > first && whole_len > stop) {
-            // the part behind this one: its block has a lower index, so it runs or has run
-            if (tid == 0) sh.ready = wait_at_least(p.flags + chain, p.splits - 1 - split, p.error);
+            if (tid == 0) sh.ready = wait_at_least(p.flags + chain, p.splits - 1 - split, whole_len - stop, p.patience);
             __syncthreads();
             get(p.ends + split * rows * a.states + row, lam);
             if (!sh.ready) {
@@ -436,11 +444,11 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
                     over_channels(dB, sh.red[warp][0], tq);
                 }
             }
+            __syncthreads();
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
                 for (int j = 0; j < J; ++j) add_to(sh.sum_a[c * J + j][tid], dA[c][j]);
-            __syncthreads();
 
             // elementwise gradients
             if (ch_ok) {
@@ -823,6 +831,11 @@ void state_scan_bwd_plan(ScanParams& p) {
     p.split_steps = (int)(each * TT);
     p.splits = (int)((chunks + each - 1) / each);
     p.batch_parts = (int)p.a.batch;
+}
+
+cudaError_t state_scan_expired_waits(unsigned long long* count, cudaStream_t st) {
+    const cudaError_t e = cudaMemcpyFromSymbolAsync(count, expired_waits, sizeof(*count), 0, cudaMemcpyDeviceToHost, st);
+    return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
 }
 
 cudaError_t state_scan_backward_launch(const ScanParams& p, cudaStream_t st) {

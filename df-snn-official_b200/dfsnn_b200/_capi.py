@@ -95,6 +95,8 @@ SIGNATURES = {
     "dfsnn_state_scan_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i, _i]),
     "dfsnn_state_scan_backward_launches": (_i, [_ll, _ll, _ll, _i, _i]),
     "dfsnn_state_scan_backward": (_i, [_args, _args, _p, _sz, _p]),
+    "dfsnn_state_scan_expired_waits": (_i, [_p, _p]),
+    "dfsnn_check_state_scan_waits": (_i, [_args, _args, _p, _sz, _p]),
     "dfsnn_state_scan_step": (_i, [_args, _p]),
     "dfsnn_short_conv_forward": (_i, [_args, _p]),
     "dfsnn_short_conv_backward_workspace_size": (_sz, [_ll, _ll, _ll, _i]),

@@ -23,6 +23,7 @@ captured into a CUDA graph.  As with any torch operation, a backward can be capt
 no eager graph of the same leaves is alive (torch makes the leaves' gradient nodes wait for the
 stream of that graph, which a capture refuses): drop such outputs first.
 """
+import ctypes
 import math
 
 import torch
@@ -317,6 +318,18 @@ def state_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=Fals
     else:
         y, last, _ = _scan_forward(*tensors, lengths, softplus, return_state, False)
     return (y, last) if return_state else y
+
+
+def expired_waits(device=None):
+    """Waits of state_scan's backward that ran out on this device since the start of the process.
+
+    For some sizes blocks of the backward wait for one another, within bounds; gradients that depend on a
+    wait that ran out are NaN.  0 unless the device stalls.  Synchronises the current stream."""
+    count = ctypes.c_ulonglong()
+    with torch.cuda.device(device):
+        _capi.check(_capi.lib().dfsnn_state_scan_expired_waits(
+            ctypes.byref(count), torch.cuda.current_stream().cuda_stream), "expired_waits")
+    return count.value
 
 
 def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, softplus=False,

@@ -439,6 +439,14 @@ int dfsnn_state_scan_backward_launches(long long T, long long batch, long long c
                                        int groups);
 int dfsnn_state_scan_backward(const dfsnn_state_scan_args* args, const dfsnn_state_scan_grads* grads,
                               void* workspace, size_t workspace_bytes, void* stream);
+/* For some sizes the parts of a sequence run one after another in one launch of the backward, and a
+ * block waits for the block of the next part.  The waits are bounded (some seconds, more for long
+ * sequences); gradients that depend on one that ran out are NaN.  Their number since the start of the
+ * process, on the current device: synchronises the stream and so takes in all calls on it. */
+int dfsnn_state_scan_expired_waits(unsigned long long* count, void* stream);
+/* Self-check: the backward with waits that run out at once. */
+int dfsnn_check_state_scan_waits(const dfsnn_state_scan_args* args, const dfsnn_state_scan_grads* grads,
+                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* One step for each of `batch` rows.  Row b reads the state at slot index[b] of `state` and
  * writes the new one to the same slot of `state_out` (`state` itself, or memory that does not

@@ -4,7 +4,7 @@ import torch
 from torch.autograd import forward_ad
 
 import state_ref
-from dfsnn_b200 import state_space as ss
+from dfsnn_b200 import _capi, state_space as ss
 from test_gpu_state_space import close, scan_case
 
 pytestmark = pytest.mark.gpu
@@ -228,3 +228,38 @@ def test_scan_parts_whose_decay_overflows():
     d, gy = delta.clone(), torch.zeros(T, 1, D, device=DEV)
     d[-64:], gy[-1] = 0.5, 1e-30
     check(torch.zeros(T, 1, D, device=DEV), d, torch.zeros(1, D, N, device=DEV), gy)
+
+
+# ---------------------------------------------------------------------------------------
+# parts that wait for one another
+# ---------------------------------------------------------------------------------------
+def test_waits_that_run_out_are_counted_and_give_nan(monkeypatch):
+    """The same backward with waits of no length: the last part of each sequence is whole, what comes in
+    front of it NaN, the call returns, and the next one is as if nothing had been."""
+    T, B, D = 300, 480, 8
+    lib = _capi.lib()
+    x, _, (gy, gh) = scan_case(T, B, D, 16, 1, "f32", seed=1, scale=0.1)
+    assert lib.dfsnn_state_scan_backward_launches(T, B, D, 16, 1) == 2
+    leaves = {k: v.detach().requires_grad_(True) for k, v in x.items()}
+
+    def run():
+        y, h = ss.state_scan(**leaves, softplus=True, return_state=True)
+        return dict(zip(leaves, torch.autograd.grad([y, h], list(leaves.values()), [gy, gh])))
+    want, before = run(), ss.expired_waits()
+    assert all(torch.isfinite(v).all() for v in want.values())
+    with monkeypatch.context() as m:
+        m.setattr(lib, "dfsnn_state_scan_backward", lib.dfsnn_check_state_scan_waits)
+        got = run()
+    # 480 sequences in two parts
+    assert ss.expired_waits() - before == B
+    last = int(torch.isnan(got["u"]).any(-1).any(-1).sum())             # steps of the first parts
+    assert 0 < last < T and last % 16 == 0
+    for k in ("u", "delta", "B"):
+        assert torch.isnan(got[k][:last]).all() and torch.equal(got[k][last:], want[k][last:]), k
+    for k in ("C", "z"):                                                # these need no later step
+        assert torch.equal(got[k], want[k]), k
+    for k in ("A", "delta_bias", "h0"):
+        assert torch.isnan(got[k]).all(), k
+    again = run()
+    assert all(torch.equal(again[k], want[k]) for k in want)
+    assert ss.expired_waits(DEV) - before == B

@@ -3,7 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from dfsnn_b200 import state_space as ss
+from dfsnn_b200 import _capi, state_space as ss
 
 
 # ---------------------------------------------------------------------------------------
@@ -53,3 +53,7 @@ def test_steps_refuse_inputs_that_require_gradients():
         ss._no_gradients("test", (x, w))
     with pytest.raises(RuntimeError, match="test is not differentiable"):
         ss._no_gradients("test", (x, None, w))
+
+
+def test_expired_waits_without_a_place():
+    assert _capi.lib().dfsnn_state_scan_expired_waits(None, None) == _capi.DFSNN_ERR_NULL
