@@ -3,7 +3,10 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+import state_bounds
+import state_ref
 from dfsnn_b200 import _capi, state_space as ss
+from test_state_space import scan_autograd, scan_inputs
 
 
 # ---------------------------------------------------------------------------------------
@@ -57,3 +60,34 @@ def test_steps_refuse_inputs_that_require_gradients():
 
 def test_expired_waits_without_a_place():
     assert _capi.lib().dfsnn_state_scan_expired_waits(None, None) == _capi.DFSNN_ERR_NULL
+
+
+# ---------------------------------------------------------------------------------------
+# the error bounds that the GPU tests go by
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("full", [True, False])
+def test_bounds_go_with_the_formulas(full):
+    """state_bounds.py has the values of state_ref.py, and fp32 evaluations of the formulas keep to its
+    bounds."""
+    g = torch.Generator().manual_seed(3)
+    x = {k: v.float() for k, v in scan_inputs(40, 3, 8, 6, 2, full, True).items()}
+    n = torch.tensor([40, 17, 0])
+    gy, gh = torch.randn(40, 3, 8, generator=g), torch.randn(3, 8, 6, generator=g)
+    want, bound = state_bounds.scan(**x, softplus=full, lengths=n, gy=gy, gh=gh)
+    ref = state_ref.scan(**x, softplus=full, lengths=n, gy=gy, gh=gh)
+    keys = ["y", "h", *("g" + k for k in x)]
+    for k in keys:
+        assert torch.allclose(want[k], ref[k], rtol=1e-12, atol=1e-13), k
+        assert (bound[k] >= 0).all() and bound[k].max() < 1e-3 * (1 + want[k].abs().max()), k
+    leaves = {k: v.clone().requires_grad_(True) for k, v in x.items()}
+    y, h = scan_autograd(leaves, full, n)
+    got = [y, h, *torch.autograd.grad([y, h], list(leaves.values()), [gy, gh])]
+    for k, v in zip(keys, got):
+        state_bounds.check(v.float(), want[k], bound[k], k)     # (padding makes y 64 bits wide)
+    w, b = torch.randn(8, 4, generator=g), torch.randn(8, generator=g)
+    s, gl = torch.randn(3, 3, 8, generator=g), torch.randn(3, 3, 8, generator=g)
+    want, bound = state_bounds.conv(x["u"], w, b, full, s, n, gy, gl)
+    ref = state_ref.conv(x["u"], w, b, full, s, n, gy, gl)
+    for k, v in want.items():
+        assert torch.allclose(v, ref[k], rtol=1e-12, atol=1e-13), k
+        assert bound[k].max() < 1e-3, k
