@@ -215,12 +215,12 @@ __global__ void __launch_bounds__(NT, 3) scan_bwd(const ScanParams p) {
         auto fill = [&](int t0) {
             const int rows = len - t0;
             Raw& r = sh.raw[t0 / TT & 1];
-            fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words, threadIdx.x);
-            fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words, threadIdx.x);
-            fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], g_p, a.y_t, rows, cols, p.words, threadIdx.x);
-            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words, threadIdx.x);
-            fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words, threadIdx.x);
-            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], g_p, a.y_t, rows, cols, p.words);
+            if (a.z) fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
+            fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
             u_p -= TT * a.u_t;
             d_p -= TT * a.delta_t;
             z_p -= TT * a.z_t;
@@ -595,11 +595,11 @@ __global__ void __launch_bounds__(NT) scan_bwd_ends(const ScanParams p) {
         const int rows = len - t0;
         const long long c = g_base + c_base;
         typename Tl::Raw& r = sh.raw[t0 / TT & 1];
-        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], static_cast<const IO*>(a.delta) + b * a.delta_b + c + t0 * a.delta_t, a.delta_t, rows, cols, p.words, threadIdx.x);
-        fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], static_cast<const IO*>(p.g.grad_y) + b * a.y_b + c + t0 * a.y_t, a.y_t, rows, cols, p.words, threadIdx.x);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.d[0], static_cast<const IO*>(a.delta) + b * a.delta_b + c + t0 * a.delta_t, a.delta_t, rows, cols, p.words);
+        fill_tile<IO, TT, BC, NT, WIDE>(r.g[0], static_cast<const IO*>(p.g.grad_y) + b * a.y_b + c + t0 * a.y_t, a.y_t, rows, cols, p.words);
         if (a.z)
-            fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], static_cast<const IO*>(a.z) + b * a.z_b + c + t0 * a.z_t, a.z_t, rows, cols, p.words, threadIdx.x);
-        fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + t0 * a.C_t, a.C_t, rows, a.states, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, WIDE>(r.z[0], static_cast<const IO*>(a.z) + b * a.z_b + c + t0 * a.z_t, a.z_t, rows, cols, p.words);
+        fill_tile<IO, TT, NS, NT, WIDE>(r.C_[0], static_cast<const IO*>(a.C) + b * a.C_b + grp * a.C_g + t0 * a.C_t, a.C_t, rows, a.states, p.words);
         copy_commit();
     };
     const int top = (len - 1) / TT * TT;

@@ -32,12 +32,11 @@ namespace {
 
 constexpr int TT = kScanTile, NT = 128;
 
-// S states on each of a channel's SL lanes, C channels a lane
-template <typename IO, int S, int SL, int C>
+// S states on each of a channel's SL lanes
+template <typename IO, int S, int SL>
 struct Tile {
-    static constexpr int CL = 32 / SL;                 // channel lanes of a warp
-    static constexpr int CW = CL * C;                  // channels of a warp
-    static constexpr int BC = NT / 32 * CW;            // channels of the block
+    static constexpr int CL = 32 / SL;                 // channels of a warp
+    static constexpr int BC = NT / 32 * CL;            // channels of the block
     static constexpr int NS = S * SL;                  // states, padded
     struct Raw {                                       // as the sequences have them
         IO u[TT][BC], d[TT][BC], z[TT][BC], B[TT][NS], C_[TT][NS];
@@ -74,10 +73,10 @@ struct __align__(sizeof(IO) * V) Pack {
     IO v[V];
 };
 
-template <typename IO, int S, int SL, int C, bool WIDE, bool ENDS>
+template <typename IO, int S, int SL, bool WIDE, bool ENDS>
 __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
-    using Tl = Tile<IO, S, SL, C>;
-    constexpr int CL = Tl::CL, CW = Tl::CW, BC = Tl::BC, NS = Tl::NS;
+    using Tl = Tile<IO, S, SL>;
+    constexpr int CL = Tl::CL, BC = Tl::BC, NS = Tl::NS, J = S / 2;
     constexpr int V = WIDE ? 2 : 1;                             // channels of a pack
     constexpr int ROW = BC / V;                                 // threads along a step's channels
     constexpr int E = TT * ROW > NT ? TT * ROW / NT : 1;        // packs of a thread,
@@ -122,15 +121,15 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     auto fill = [&](int t0) {
         const int stage = fetched++ & 1, rows = len_ahead - t0;
         if constexpr (WIDE) {
-            pieces.template issue<Tl::kEights, 1>(stage * (unsigned)sizeof(Raw), rows);
+            pieces.template issue<Tl::kEights>(stage * (unsigned)sizeof(Raw), rows);
         } else {
             Raw& r = sh.raw[stage];
-            fill_tile<IO, TT, BC, NT, false>(r.u[0], u_p, a.u_t, rows, cols, p.words, threadIdx.x);
-            fill_tile<IO, TT, BC, NT, false>(r.d[0], d_p, a.delta_t, rows, cols, p.words, threadIdx.x);
-            fill_tile<IO, TT, NS, NT, false>(r.B[0], B_p, a.B_t, rows, a.states, p.words, threadIdx.x);
+            fill_tile<IO, TT, BC, NT, false>(r.u[0], u_p, a.u_t, rows, cols, p.words);
+            fill_tile<IO, TT, BC, NT, false>(r.d[0], d_p, a.delta_t, rows, cols, p.words);
+            fill_tile<IO, TT, NS, NT, false>(r.B[0], B_p, a.B_t, rows, a.states, p.words);
             if (!ENDS) {
-                if (a.z) fill_tile<IO, TT, BC, NT, false>(r.z[0], z_p, a.z_t, rows, cols, p.words, threadIdx.x);
-                fill_tile<IO, TT, NS, NT, false>(r.C_[0], C_p, a.C_t, rows, a.states, p.words, threadIdx.x);
+                if (a.z) fill_tile<IO, TT, BC, NT, false>(r.z[0], z_p, a.z_t, rows, cols, p.words);
+                fill_tile<IO, TT, NS, NT, false>(r.C_[0], C_p, a.C_t, rows, a.states, p.words);
             }
             u_p += TT * a.u_t;
             d_p += TT * a.delta_t;
@@ -163,42 +162,33 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     };
     open(b0);                                                   // in flight while the states are set up
 
-    // recurrence role: states n0 .. n0 + S - 1 of channels cl + c * CL of the block
-    const int sl = lane / CL, cl = warp * CW + lane % CL, n0 = sl * S;
-    const long long crow = (long long)CL * a.states;            // from one channel of a lane to the next
+    // recurrence role: states n0 .. n0 + S - 1 of channel cl of the block
+    const int sl = lane / CL, cl = warp * CL + lane % CL, n0 = sl * S;
+    auto cl_ok = [&]() { return c_base + cl < p.group_channels; };
     // a lane's states are one 16-byte access everywhere
     const bool whole = S == 4 && a.states % 4 == 0
                        && ((reinterpret_cast<uintptr_t>(a.kept) | reinterpret_cast<uintptr_t>(a.h_last)) & 15) == 0;
-    float2 A2[C][S / 2] = {}, h[C][S / 2] = {};
-    auto cl_ok = [&](int c) { return c_base + cl + c * CL < p.group_channels; };
-    auto get = [&](const float* q, float2(&v)[C][S / 2]) {
+    float2 A2[J] = {}, h[J] = {};
+    auto get = [&](const float* q, float2(&v)[J]) {
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const float f = q && cl_ok(c) && n0 + s < a.states ? q[c * crow + s] : 0.0f;
-                (s % 2 ? v[c][s / 2].y : v[c][s / 2].x) = f;
-            }
+        for (int s = 0; s < S; ++s) {
+            const float f = q && cl_ok() && n0 + s < a.states ? q[s] : 0.0f;
+            (s % 2 ? v[s / 2].y : v[s / 2].x) = f;
+        }
     };
     auto put = [&](float* q) {
+        if (!cl_ok() || n0 >= a.states) return;
+        if (S == 4 && whole) {
+            *reinterpret_cast<float4*>(q) = make_float4(h[0].x, h[0].y, h[J - 1].x, h[J - 1].y);
+        } else {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            if (!cl_ok(c) || n0 >= a.states) continue;
-            if (S == 4 && whole) {
-                *reinterpret_cast<float4*>(q + c * crow) =
-                    make_float4(h[c][0].x, h[c][0].y, h[c][S / 2 - 1].x, h[c][S / 2 - 1].y);
-            } else {
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-                    if (n0 + s < a.states) q[c * crow + s] = s % 2 ? h[c][s / 2].y : h[c][s / 2].x;
-            }
+            for (int s = 0; s < S; ++s)
+                if (n0 + s < a.states) q[s] = s % 2 ? h[s / 2].y : h[s / 2].x;
         }
     };
     get(a.A + (g_base + c_base + cl) * a.states + n0, A2);
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int j = 0; j < S / 2; ++j) A2[c][j] = make_float2(log2_rate(A2[c][j].x), log2_rate(A2[c][j].y));
+    for (int j = 0; j < J; ++j) A2[j] = make_float2(log2_rate(A2[j].x), log2_rate(A2[j].y));
 
     for (long long b = b0; b < a.batch; b += p.seq_blocks) {
     const int whole_len = seq_length(a.lengths, a.lengths64, b, p.T), len = whole_len < stop ? whole_len : stop;
@@ -210,21 +200,17 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
         get(a.h0 ? a.h0 + row : nullptr, h);
         const long long rows = a.batch * a.channels;
         for (int k = 0; k != split; ++k) {
-            float2 end[C][S / 2] = {};
+            float2 end[J] = {};
             get(p.ends + k * rows * a.states + row, end);
+            const float half = cl_ok() ? 0.5f * p.end_steps[k * rows + b * a.channels + g_base + c_base + cl] : 0.0f;
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const float half = cl_ok(c) ? 0.5f * p.end_steps[k * rows + b * a.channels + g_base + c_base + cl + c * CL] : 0.0f;
-#pragma unroll
-                for (int j = 0; j < S / 2; ++j)
-                    h[c][j] = make_float2(carry_over(half * A2[c][j].x, h[c][j].x, end[c][j].x),
-                                          carry_over(half * A2[c][j].y, h[c][j].y, end[c][j].y));
-            }
+            for (int j = 0; j < J; ++j)
+                h[j] = make_float2(carry_over(half * A2[j].x, h[j].x, end[j].x), carry_over(half * A2[j].y, h[j].y, end[j].y));
         }
     } else if (split == 0) {
         get(a.h0 ? a.h0 + row : nullptr, h);                    // an empty sequence keeps its state
     }
-    float steps[C] = {};                                        // sums of d
+    float steps = 0.0f;                                         // sum of d
     const long long all_states = a.batch * a.channels * a.states;
     float* kept = a.kept + row - all_states;                    // of step t at t / R * all_states
 
@@ -258,32 +244,28 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
         }
         __syncthreads();
         // decays that stay near 1 for the whole tile take the polynomial
-        bool near1[C][S];
+        bool near1[S];
+        float most = 0.0f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float most = 0.0f;
+        for (int t = 0; t < TT; t += SL)
+            if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d(cl)[t + (SL <= TT ? sl : sl % TT)].x));
 #pragma unroll
-            for (int t = 0; t < TT; t += SL)
-                if (SL <= TT || sl < TT) most = fmaxf(most, fabsf(sh.d(cl + c * CL)[t + (SL <= TT ? sl : sl % TT)].x));
+        for (int m = SL / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m * CL));
 #pragma unroll
-            for (int m = SL / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m * CL));
-#pragma unroll
-            for (int j = 0; j < S / 2; ++j) {
-                near1[c][2 * j] = most * fabsf(A2[c][j].x) < kExp2Near;
-                near1[c][2 * j + 1] = most * fabsf(A2[c][j].y) < kExp2Near;
-            }
+        for (int j = 0; j < J; ++j) {
+            near1[2 * j] = most * fabsf(A2[j].x) < kExp2Near;
+            near1[2 * j + 1] = most * fabsf(A2[j].y) < kExp2Near;
         }
         constexpr int R = 8;                    // steps whose sums over the lanes are formed together
         constexpr int G = 2;                    // steps whose operands are read one group ahead
         static_assert(R == kScanChunk, "states are kept in front of every R steps");
-        float2 d_n[G][C], B_n[G][S / 2], C_n[G][S / 2];
+        float2 d_n[G], B_n[G][J], C_n[G][J];
         auto read = [&](int t0g) {
 #pragma unroll
             for (int t = 0; t < G; ++t) {
                 load_states<S>(B_n[t], &sh.B[t0g + t][n0]);
                 if (!ENDS) load_states<S>(C_n[t], &sh.C_[t0g + t][n0]);
-#pragma unroll
-                for (int c = 0; c < C; ++c) d_n[t][c] = sh.d(cl + c * CL)[t0g + t];
+                d_n[t] = sh.d(cl)[t0g + t];
             }
         };
         read(0);
@@ -291,59 +273,50 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
         for (int tr = 0; tr < TT; tr += R) {
             if (!ENDS && a.kept && t0 + tr > 0 && t0 + tr < len)
                 put(kept + (long long)((t0 + tr) / R) * all_states);
-            float y[C][R];
+            float y[R];
 #pragma unroll
             for (int tg = 0; tg < R; tg += G) {
-                float2 d_c[G][C], B_c[G][S / 2], C_c[G][S / 2];
+                float2 d_c[G], B_c[G][J], C_c[G][J];
 #pragma unroll
                 for (int t = 0; t < G; ++t) {
+                    d_c[t] = d_n[t];
 #pragma unroll
-                    for (int c = 0; c < C; ++c) d_c[t][c] = d_n[t][c];
-#pragma unroll
-                    for (int j = 0; j < S / 2; ++j) {
+                    for (int j = 0; j < J; ++j) {
                         B_c[t][j] = B_n[t][j];
                         if (!ENDS) C_c[t][j] = C_n[t][j];
                     }
                 }
                 if (tr + tg + G < TT) read(tr + tg + G);
-                float2 dec[G][C][S / 2], in[G][C][S / 2];
+                float2 dec[G][J], in[G][J];
 #pragma unroll
-                for (int t = 0; t < G; ++t)
+                for (int t = 0; t < G; ++t) {
+                    const float2 dt = make_float2(d_c[t].x, d_c[t].x), du = make_float2(d_c[t].y, d_c[t].y);
+                    if (ENDS) steps += d_c[t].x;
 #pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        const float2 d = d_c[t][c];
-                        const float2 dt = make_float2(d.x, d.x), du = make_float2(d.y, d.y);
-                        if (ENDS) steps[c] += d.x;
-#pragma unroll
-                        for (int j = 0; j < S / 2; ++j) {
-                            const float2 x = __fmul2_rn(dt, A2[c][j]), q = exp2_near1(x);
-                            dec[t][c][j] = make_float2(near1[c][2 * j] ? q.x : exp2_approx(x.x),
-                                                       near1[c][2 * j + 1] ? q.y : exp2_approx(x.y));
-                            in[t][c][j] = __fmul2_rn(du, B_c[t][j]);
-                        }
+                    for (int j = 0; j < J; ++j) {
+                        const float2 x = __fmul2_rn(dt, A2[j]), q = exp2_near1(x);
+                        dec[t][j] = make_float2(near1[2 * j] ? q.x : exp2_approx(x.x),
+                                                near1[2 * j + 1] ? q.y : exp2_approx(x.y));
+                        in[t][j] = __fmul2_rn(du, B_c[t][j]);
                     }
+                }
 #pragma unroll
-                for (int t = 0; t < G; ++t)
+                for (int t = 0; t < G; ++t) {
+                    float2 acc;
 #pragma unroll
-                    for (int c = 0; c < C; ++c) {
-                        float2 acc;
-#pragma unroll
-                        for (int j = 0; j < S / 2; ++j) {
-                            h[c][j] = __ffma2_rn(dec[t][c][j], h[c][j], in[t][c][j]);
-                            if (!ENDS) acc = j == 0 ? __fmul2_rn(h[c][j], C_c[t][j]) : __ffma2_rn(h[c][j], C_c[t][j], acc);
-                        }
-                        if (!ENDS) y[c][tg + t] = acc.x + acc.y;
+                    for (int j = 0; j < J; ++j) {
+                        h[j] = __ffma2_rn(dec[t][j], h[j], in[t][j]);
+                        if (!ENDS) acc = j == 0 ? __fmul2_rn(h[j], C_c[t][j]) : __ffma2_rn(h[j], C_c[t][j], acc);
                     }
+                    if (!ENDS) y[tg + t] = acc.x + acc.y;
+                }
             }
             if (!ENDS) {
                 using Sums = LaneSums<R, SL, CL>;
+                Sums::run(y, sl);
+                if (Sums::stores(sl)) {
 #pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    Sums::run(y[c], sl);
-                    if (Sums::stores(sl)) {
-#pragma unroll
-                        for (int i = 0; i < Sums::kHeld; ++i) sh.o[cl + c * CL][tr + Sums::first(sl) + i] = y[c][i];
-                    }
+                    for (int i = 0; i < Sums::kHeld; ++i) sh.o[cl][tr + Sums::first(sl) + i] = y[i];
                 }
             }
         }
@@ -373,10 +346,7 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     if (first >= len && another) open(b + p.seq_blocks);
     if (ENDS) {
         put(p.ends + split * a.batch * a.channels * a.states + row);
-#pragma unroll
-        for (int c = 0; c < C; ++c)
-            if (cl_ok(c) && sl == 0)
-                p.end_steps[(split * a.batch + b) * a.channels + g_base + c_base + cl + c * CL] = steps[c];
+        if (cl_ok() && sl == 0) p.end_steps[(split * a.batch + b) * a.channels + g_base + c_base + cl] = steps;
         return;
     }
     // rows behind the end (y_p is at the tile behind the last)
@@ -392,21 +362,21 @@ __global__ void __launch_bounds__(NT, 5) scan_fwd(const ScanParams p) {
     }
 }
 
-template <typename IO, int S, int SL, int C, bool WIDE>
+template <typename IO, int S, int SL, bool WIDE>
 cudaError_t launch_form(const ScanParams& p, unsigned blocks, cudaStream_t st) {
-    constexpr size_t smem = sizeof(Tile<IO, S, SL, C>);
-    cudaError_t e = allow_shared<scan_fwd<IO, S, SL, C, WIDE, false>>(smem);
-    if (e == cudaSuccess && p.splits > 1) e = allow_shared<scan_fwd<IO, S, SL, C, WIDE, true>>(smem);
+    constexpr size_t smem = sizeof(Tile<IO, S, SL>);
+    cudaError_t e = allow_shared<scan_fwd<IO, S, SL, WIDE, false>>(smem);
+    if (e == cudaSuccess && p.splits > 1) e = allow_shared<scan_fwd<IO, S, SL, WIDE, true>>(smem);
     if (e != cudaSuccess) return e;
     if (p.splits > 1)
-        scan_fwd<IO, S, SL, C, WIDE, true><<<blocks * (p.splits - 1), NT, smem, st>>>(p);
-    scan_fwd<IO, S, SL, C, WIDE, false><<<blocks * p.splits, NT, smem, st>>>(p);
+        scan_fwd<IO, S, SL, WIDE, true><<<blocks * (p.splits - 1), NT, smem, st>>>(p);
+    scan_fwd<IO, S, SL, WIDE, false><<<blocks * p.splits, NT, smem, st>>>(p);
     return cudaGetLastError();
 }
 
-template <typename IO, int S, int SL, int C>
+template <typename IO, int S, int SL>
 cudaError_t launch(ScanParams p, cudaStream_t st) {
-    constexpr int BC = Tile<IO, S, SL, C>::BC;
+    constexpr int BC = Tile<IO, S, SL>::BC;
     p.tiles = (p.group_channels + BC - 1) / BC;
     // Short sequences: one wave of blocks (five an SM) takes them all, several a block, so that the
     // set-up is paid once and the next sequence is fetched meanwhile (16 steps, 4096 sequences, 256
@@ -418,29 +388,29 @@ cudaError_t launch(ScanParams p, cudaStream_t st) {
     if (blocks > 0x7fffffffLL / p.splits) return cudaErrorInvalidValue;
     const dfsnn_state_scan_args& a = p.a;
     p.words = rows_aligned(p, sizeof(IO), 4);
-    return p.group_channels % 2 == 0 && pairs_aligned(a.y, a.y_t, a.y_b, sizeof(IO)) && rows_aligned(p, sizeof(IO), 16) ? launch_form<IO, S, SL, C, true>(p, (unsigned)blocks, st)
-                                                    : launch_form<IO, S, SL, C, false>(p, (unsigned)blocks, st);
+    return p.group_channels % 2 == 0 && pairs_aligned(a.y, a.y_t, a.y_b, sizeof(IO)) && rows_aligned(p, sizeof(IO), 16) ? launch_form<IO, S, SL, true>(p, (unsigned)blocks, st)
+                                                    : launch_form<IO, S, SL, false>(p, (unsigned)blocks, st);
 }
 
 template <typename IO>
 cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     const int n = p.a.states;
-    if (n <= 4) return launch<IO, 2, 2, 1>(p, st);
-    if (n <= 8) return launch<IO, 2, 4, 1>(p, st);
-    if (n <= 16) return launch<IO, 4, 4, 1>(p, st);
-    if (n <= 32) return launch<IO, 4, 8, 1>(p, st);
-    if (n <= 64) return launch<IO, 4, 16, 1>(p, st);
-    return launch<IO, 4, 32, 1>(p, st);
+    if (n <= 4) return launch<IO, 2, 2>(p, st);
+    if (n <= 8) return launch<IO, 2, 4>(p, st);
+    if (n <= 16) return launch<IO, 4, 4>(p, st);
+    if (n <= 32) return launch<IO, 4, 8>(p, st);
+    if (n <= 64) return launch<IO, 4, 16>(p, st);
+    return launch<IO, 4, 32>(p, st);
 }
 
 // Channels of a block, as pick() has them
 int block_channels(int states) {
-    if (states <= 4) return Tile<float, 2, 2, 1>::BC;
-    if (states <= 8) return Tile<float, 2, 4, 1>::BC;
-    if (states <= 16) return Tile<float, 4, 4, 1>::BC;
-    if (states <= 32) return Tile<float, 4, 8, 1>::BC;
-    if (states <= 64) return Tile<float, 4, 16, 1>::BC;
-    return Tile<float, 4, 32, 1>::BC;
+    if (states <= 4) return Tile<float, 2, 2>::BC;
+    if (states <= 8) return Tile<float, 2, 4>::BC;
+    if (states <= 16) return Tile<float, 4, 4>::BC;
+    if (states <= 32) return Tile<float, 4, 8>::BC;
+    if (states <= 64) return Tile<float, 4, 16>::BC;
+    return Tile<float, 4, 32>::BC;
 }
 
 }  // namespace

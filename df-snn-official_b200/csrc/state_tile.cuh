@@ -19,21 +19,19 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int LEFT>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 
-// A tile of ROWS steps x COLS neighbouring elements, by NT threads of a block (`thread`: which
-// of them): steps from
-// `rows` and elements from `cols` on become zero and are not read.  WIDE: rows start on 16-byte
+// A tile of ROWS steps x COLS neighbouring elements, by the NT threads of a block: steps from `rows`
+// and elements from `cols` on become zero and are not read.  WIDE: rows start on 16-byte
 // boundaries and are copied 16 bytes at a time (8 where a row of the tile has no more).  Otherwise
 // `words` says that every row starts on a 4-byte boundary; rows that do not (odd offsets of 16-bit
 // types) are loaded and stored.
 template <typename IO, int ROWS, int COLS, int NT, bool WIDE>
-__device__ __forceinline__ void fill_tile(IO* dst, const IO* src, long long stride, int rows, int cols, bool words,
-                                          int thread) {
+__device__ __forceinline__ void fill_tile(IO* dst, const IO* src, long long stride, int rows, int cols, bool words) {
     constexpr int E = (int)sizeof(IO);
     constexpr int BYTES = !WIDE ? 4 : COLS * E >= 16 ? 16 : COLS * E;
     constexpr int PER = BYTES / E, CPR = COLS / PER;
     if (WIDE || words) {
 #pragma unroll 4
-        for (int i = thread; i < ROWS * CPR; i += NT) {
+        for (int i = threadIdx.x; i < ROWS * CPR; i += NT) {
             const int t = i / CPR, c = i % CPR * PER;
             int n = t < rows ? (cols - c) * E : 0;
             n = n < 0 ? 0 : n > BYTES ? BYTES : n;
@@ -41,7 +39,7 @@ __device__ __forceinline__ void fill_tile(IO* dst, const IO* src, long long stri
         }
     } else {
 #pragma unroll 4
-        for (int i = thread; i < ROWS * COLS; i += NT) {
+        for (int i = threadIdx.x; i < ROWS * COLS; i += NT) {
             const int t = i / COLS, c = i % COLS;
             dst[i] = t < rows && c < cols ? src[t * stride + c] : from_f<IO>(0.0f);
         }
@@ -88,9 +86,8 @@ struct TilePieces {
         }
         next += ROWS * CPR;
     }
-    // copies of the current tile to the stage `offset` bytes on, and on to the next tile (DIRECTION
-    // 1) or the one in front (-1)
-    template <bool EIGHTS, int DIRECTION>
+    // copies of the current tile to the stage `offset` bytes on, and on to the next tile
+    template <bool EIGHTS>
     __device__ __forceinline__ void issue(unsigned offset, int rows) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -100,7 +97,7 @@ struct TilePieces {
                     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst[k] + offset), "l"(src[k]), "r"(bytes) : "memory");
                 else
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst[k] + offset), "l"(src[k]), "r"(bytes) : "memory");
-                src[k] += DIRECTION * step[k];
+                src[k] += step[k];
             }
         }
     }
