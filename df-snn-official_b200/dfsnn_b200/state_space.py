@@ -170,9 +170,11 @@ def _no_tangents(name, tensors):
 
 def _no_gradients(name, tensors):
     """Refuses what a step form could only cut off from its graph, as torch does for `out=`."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is not differentiable, but an input requires a gradient: call it under "
-                           "torch.no_grad(), or the sequence form with one step")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} is not differentiable, but an input requires a gradient: call it "
+                                   "under torch.no_grad(), or the sequence form with one step")
 
 
 # ---------------------------------------------------------------------------------------
@@ -357,9 +359,9 @@ def state_scan_step(u, delta, state, A, B, C, D=None, z=None, delta_bias=None, s
     D = _param(D, dev, (Dn,), name, "D")
     bias = _param(delta_bias, dev, (Dn,), name, "delta_bias")
     index = _integers(index, dev, Bn, name, "index")
-    tensors = (u, delta, A, B, C, D, z, bias)
-    _no_gradients(name, tensors)
-    _no_tangents(name, (*tensors, state))
+    _no_gradients(name, (u, delta, A, B, C, D, z, bias))
+    if _fw._current_level >= 0:
+        _no_tangents(name, (u, delta, A, B, C, D, z, bias, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, torch.float32, dev, (Dn, N), Bn, index, name)
     y = u.new_empty(shape)
     args = _capi.STATE_SCAN_STEP_ARGS.pack(
@@ -472,7 +474,8 @@ def short_conv_step(x, state, weight, bias=None, activation=None, index=None, st
     bias = _param(bias, dev, (Dn,), name, "bias")
     index = _integers(index, dev, Bn, name, "index")
     _no_gradients(name, (x, weight, bias))
-    _no_tangents(name, (x, weight, bias, state))
+    if _fw._current_level >= 0:
+        _no_tangents(name, (x, weight, bias, state))
     state_out, slots, s_in, s_out = _pool(state, state_out, dtype, dev, (W - 1, Dn), Bn, index, name)
     y = x.new_empty(shape)
     args = _capi.SHORT_CONV_STEP_ARGS.pack(
