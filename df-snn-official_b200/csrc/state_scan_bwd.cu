@@ -11,12 +11,12 @@
 // other lanes; grad B and grad C), both formed for 4 steps at a time (LaneSums).  Packed pairs of
 // states halve the arithmetic's issue slots; elementwise work is done once per (step, channel) by
 // all threads.  The sums over channels go on over the warps in shared memory and over the blocks
-// through partial sums that a second kernel adds in a fixed order: no atomics, so results do not
+// through partial sums that a second kernel adds in a fixed order: no atomic sums, so results do not
 // change from run to run.
 //
-// Bound by instruction issue (58 % of the slots) and the shared-memory pipe (66 %) together, at
-// three blocks an SM: T = 2048, 8 sequences, 2048 channels, bf16, N = 16: 891 us, 537 M (step,
-// channel, state) at 0.60 T/s.  Four states on a lane and one channel: two channels a lane halve the
+// Bound by instruction issue (58 % of the slots) and the shared-memory pipe (69 %) together, at
+// three blocks an SM: T = 2048, 8 sequences, 2048 channels, bf16, N = 16: 893 us (the second kernel 30),
+// 537 M (step, channel, state) at 0.60 T/s.  Four states on a lane and one channel: two channels a lane halve the
 // shuffles of the sums over channels, but leave 8 warps an SM (1150 us).
 #include <algorithm>
 #include <type_traits>
@@ -786,7 +786,10 @@ cudaError_t pick(const ScanParams& p, cudaStream_t st) {
     return cudaGetLastError();
 }
 
-// Channels of a block for a state count, as pick() has them
+// Channels of a block for a state count, as pick() has them.  N = 5 .. 8: two channels a lane, which is
+// better for short sequences (fp32, 16 x 4096 x 256: 317 us against 333 with one) and few rows (bf16,
+// 1000 x 4 x 1000: 143 against 154), not for long ones that fill the machine (fp32, 1024 x 8 x 2048: 477
+// against 326).
 int block_channels(int states) {
     if (states <= 4) return Tile<float, 2, 2, 1>::BC;
     if (states <= 8) return Tile<float, 2, 4, 2>::BC;
@@ -804,13 +807,14 @@ int state_scan_bwd_tiles(int states, long long group_channels) {
 }
 
 // How the blocks share sequences, of which `slots` walk one at a time (three blocks on each of 148
-// SMs).  bf16, N = 16, microseconds with the rule and without:
+// SMs; for N > 64 the blocks' shared memory leaves two, one in fp32, and the rule was not measured
+// there).  bf16, N = 16, microseconds of the whole backward with the rule and without:
 //   * few rows (two parts a sequence fit the slots): each sequence in parts side by side, at the
 //     price of a second walk for their ends: 4096 x 1 x 512 91 against 940, 4096 x 1 x 4096 665
 //     against 984; parts of 4 tiles at least;
 //   * more blocks than slots: the last wave of blocks would leave most of the machine idle for a
 //     whole walk.  The sequences are cut into parts that run one after another, a block passing its
-//     a_t l_t on to the next (chained), so that the last wave is a short one: 2048 x 8 x 2048 922
+//     a_t l_t on to the next (chained), so that the last wave is a short one: 2048 x 8 x 2048 924
 //     against 1205, 512 x 8 x 2048 261 against 323;
 //   * 8 blocks an SM are enough of them: beyond that a block takes several sequences and adds its
 //     grad A on the way, which keeps the partial sums small.

@@ -14,8 +14,8 @@
 //   * the operands of a group of steps are read from shared memory while the group before runs.
 // States, decays and sums are fp32; y is rounded once.
 //
-// T = 2048, 8 sequences, 2048 channels, bf16, N = 16, gated: 327 us, 537 M (step, channel, state) at
-// 1.64 T/s (36 % of the special-function unit's rate; issue and the shared-memory pipe are 57 %
+// T = 2048, 8 sequences, 2048 channels, bf16, N = 16, gated: 332 us, 537 M (step, channel, state) at
+// 1.62 T/s (36 % of the special-function unit's rate; issue and the shared-memory pipe are 57 %
 // busy at 13 warps an SM); with 32 sequences 2.05 T/s.
 //
 // Few rows leave most of the machine idle, so a long sequence is then cut into `splits` parts that
